@@ -200,6 +200,11 @@ int thvm_hip_program_check(const char *name, const char *program);
 int thvm_hip_attn_decode_noalloc(const char *program, const uint32_t *buf_ids,
                                  uint32_t n_args);
 
+/* Bytes of workspace (the last buffer) that an attn_paged builtin with this
+ * spec takes: `program` is the "thvm-builtin:attn_paged ..." text.  Needs no
+ * device; 0 when the spec would be refused (thvm_hip_last_error says why). */
+uint64_t thvm_hip_attn_paged_ws(const char *program);
+
 /* ===================== renderer target ================================= */
 /* One node of a kernel's lifted uop DAG, flattened for the C ABI, sources
  * before users.  `op` is the reference's UOP_* number (src/thvm.h:302-512);

@@ -109,6 +109,7 @@ _SIGS = {
     "thvm_hip_dispatch_custom": (_i32, [_cp, _cp, _vp, _vp, _u32, _vp, _u32, _u64]),
     "thvm_hip_program_check": (_i32, [_cp, _cp]),
     "thvm_hip_attn_decode_noalloc": (_i32, [_cp, _vp, _u32]),
+    "thvm_hip_attn_paged_ws": (_u64, [_cp]),
     "thvm_hip_render_kernel": (_i32, [C.POINTER(Uop), _u32, _cp, _vp, _u64, C.POINTER(RenderInfo)]),
     "thvm_hip_render_kernel_opts": (_i32, [C.POINTER(Uop), _u32, _cp, C.POINTER(RenderOpts), _vp, _u64,
                                            C.POINTER(RenderInfo)]),
@@ -246,11 +247,24 @@ def dispatch(name: str, program: str, args, grid=(1, 1, 1), block=(1, 1, 1), sha
            f"dispatch {name}")
 
 
+def builtin_program(kernel: str, **params) -> str:
+    """The program text of a built-in gfx950 kernel: "thvm-builtin:<kernel> k=v ..."."""
+    toks = [f"{k}={float(v).hex() if isinstance(v, float) else int(v)}" for k, v in params.items()]
+    return "thvm-builtin:" + kernel + (" " + " ".join(toks) if toks else "")
+
+
 def builtin(kernel: str, args, outs=(0,), **params) -> None:
     """Fire a built-in gfx950 kernel: program "thvm-builtin:<kernel> k=v ..."."""
-    toks = [f"{k}={float(v).hex() if isinstance(v, float) else int(v)}" for k, v in params.items()]
-    dispatch(kernel, "thvm-builtin:" + kernel + (" " + " ".join(toks) if toks else ""), args,
-             outs=outs)
+    dispatch(kernel, builtin_program(kernel, **params), args, outs=outs)
+
+
+def attn_paged_ws(**params) -> int:
+    """Bytes of the workspace buffer that the attn_paged builtin takes with
+    these parameters; needs no device."""
+    nbytes = lib().thvm_hip_attn_paged_ws(builtin_program("attn_paged", **params).encode())
+    if nbytes == 0:
+        raise ThvmHipError(f"attn_paged_ws: {last_error()}")
+    return nbytes
 
 
 class Jit:

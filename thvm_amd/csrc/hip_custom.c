@@ -14,6 +14,7 @@
  */
 #define _GNU_SOURCE
 #include "internal.h"
+#include "paged_check.h"
 
 #include <hip/hiprtc.h>
 #include <errno.h>
@@ -171,6 +172,110 @@ static int attn_parse(const Spec *sp, ArgCtx *c, ThvmAttnArgs *a, int with_part)
    * merge blocks: 2 x blocks x 10 u64) */
   if (with_part && a->clk_cap) a->clk = (uint64_t *)arg(c, 6, (u64)a->clk_cap * 2 * 80);
   return c->bad ? -1 : 0;
+}
+
+/* ---- the paged-cache builtins (kv_append, kv_read, attn_paged) ---- */
+static int paged_op(const char *kernel) {
+  return strcmp(kernel, "kv_append") == 0 ? PG_APPEND : strcmp(kernel, "kv_read") == 0 ? PG_READ
+       : strcmp(kernel, "attn_paged") == 0 ? PG_ATTN : -1;
+}
+
+/* the spec's numbers, checked (no device, no buffers) */
+static int paged_parse(const Spec *sp, int op, ThvmPagedArgs *a) {
+  memset(a, 0, sizeof *a);
+  if (spec_u32(sp, "n", &a->n, 1, 0) || spec_u32(sp, "b", &a->b, 1, 0) || spec_u32(sp, "hkv", &a->Hkv, 1, 0) ||
+      spec_u32(sp, "hd", &a->hd, 1, 0) || spec_u32(sp, "page", &a->page, 1, 0) ||
+      spec_u32(sp, "maxpages", &a->maxpages, 1, 0) || spec_u32(sp, "npages", &a->npages, 1, 0) ||
+      spec_u32(sp, "dt", &a->dt, 0, THVM_DT_BF16) || spec_u32(sp, "bits", &a->bits, 0, 16) ||
+      spec_u32(sp, "ragged", &a->ragged, 0, 0) || spec_u32(sp, "h", &a->H, op != PG_READ, 0))
+    return -1;
+  if (op == PG_APPEND &&
+      (spec_u32(sp, "rope", &a->rope, 0, 0) || spec_u32(sp, "norm", &a->norm, 0, 0) ||
+       spec_f32(sp, "eps", &a->eps, 0, 1e-6f) || spec_u32(sp, "ldx", &a->ldx, 0, (a->H + 2 * a->Hkv) * a->hd)))
+    return -1;
+  if (op == PG_ATTN &&
+      (spec_f32(sp, "scale", &a->scale, 1, 0) ||
+       spec_u32(sp, "t", &a->t, 0, a->ragged || a->b == 0 ? a->n : a->n / a->b)))
+    return -1;
+  char err[200];
+  if (pg_check(a, op, err, sizeof err)) { hb_set_error("builtin %s: %s", sp->kernel, err); return -1; }
+  return 0;
+}
+
+/* The buffer slots: outputs first, then the inputs.  Rows are moved 16 bytes at
+ * a time, and blocks write while others read: pointers are aligned, and no
+ * output shares bytes with another argument. */
+static int paged_args(ArgCtx *c, int op, ThvmPagedArgs *a) {
+  struct { const char *p; u64 n; u32 slot; } r[16];
+  u32 nr = 0, slot = 0, n_out = 0;
+#define PG_ARG(field, bytes, al) do {                                                                         \
+    const u64 nb_ = (bytes);                                                                                  \
+    char *p_ = (char *)arg(c, slot, nb_);                                                                     \
+    if (!p_) return -1;                                                                                       \
+    if ((uintptr_t)p_ % (al)) { hb_set_error("builtin %s: argument %u is not %u-byte aligned", c->k, slot, (u32)(al)); return -1; } \
+    r[nr].p = p_; r[nr].n = nb_; r[nr].slot = slot; nr++; slot++;                                             \
+    a->field = (void *)p_;                                                                                    \
+  } while (0)
+  const u64 n = a->n, qb = n * a->H * a->hd * 2, kvb = n * a->Hkv * a->hd * 2, pool = pg_pool_bytes(a);
+  if (op == PG_APPEND) {
+    PG_ARG(q, qb, 16);
+    PG_ARG(kpages, pool, 16);
+    PG_ARG(vpages, pool, 16);
+    n_out = 3;
+    PG_ARG(x, ((n - 1) * a->ldx + (u64)(a->H + 2 * a->Hkv) * a->hd) * 2, 16);
+  } else if (op == PG_READ) {
+    PG_ARG(k, kvb, 16);
+    PG_ARG(v, kvb, 16);
+    n_out = 2;
+    PG_ARG(kpages, pool, 16);
+    PG_ARG(vpages, pool, 16);
+  } else {
+    PG_ARG(out, qb, 16);
+    n_out = 1;
+    PG_ARG(q, qb, 16);
+    PG_ARG(kpages, pool, 16);
+    PG_ARG(vpages, pool, 16);
+  }
+  PG_ARG(table, (u64)a->b * a->maxpages * 4, 4);
+  PG_ARG(len, (u64)a->b * 4, 4);
+  if (a->ragged) PG_ARG(rows, ((u64)a->b + 1) * 4, 4);
+  if (op == PG_APPEND && a->norm) {
+    PG_ARG(gq, (u64)a->hd * 4, 16);
+    PG_ARG(gk, (u64)a->hd * 4, 16);
+  }
+  if (op == PG_APPEND && a->rope) {
+    const u64 tb = (u64)a->maxpages * a->page * (a->hd / 2) * 4;
+    PG_ARG(cos_t, tb, 16);
+    PG_ARG(sin_t, tb, 16);
+  }
+  if (op == PG_ATTN) {                               /* the workspace is written too */
+    const u64 wsb = thvm_k_attn_paged_ws(a);
+    PG_ARG(ws, wsb, 16);
+  }
+#undef PG_ARG
+  for (u32 i = 0; i < nr; i++)
+    for (u32 j = 0; j < nr; j++)
+      if (i != j && (i < n_out || (op == PG_ATTN && i == nr - 1)) && r[i].p < r[j].p + r[j].n && r[j].p < r[i].p + r[i].n) {
+        hb_set_error("builtin %s: argument %u is written and shares bytes with argument %u", c->k, r[i].slot, r[j].slot);
+        return -1;
+      }
+  return 0;
+}
+
+THVM_API uint64_t thvm_hip_attn_paged_ws(const char *program) {
+  Spec sp;
+  ThvmPagedArgs a;
+  if (!program || strncmp(program, BUILTIN_PREFIX, strlen(BUILTIN_PREFIX)) != 0) {
+    hb_set_error("attn_paged_ws: want a thvm-builtin:attn_paged program");
+    return 0;
+  }
+  if (spec_parse(program, &sp)) return 0;
+  if (paged_op(sp.kernel) != PG_ATTN) {
+    hb_set_error("attn_paged_ws: program is thvm-builtin:%s, want thvm-builtin:attn_paged", sp.kernel);
+    return 0;
+  }
+  if (paged_parse(&sp, PG_ATTN, &a)) return 0;
+  return thvm_k_attn_paged_ws(&a);
 }
 
 /* Launch (or only validate, check_only=1) a builtin program. */
@@ -338,6 +443,18 @@ int hb_builtin_launch(const char *program, const u32 *ids, u32 n, int check_only
     if (check_only) return 0;
     if (prof) hb_kprof_begin(K, &e0, &e1);
     rc = thvm_k_attn_prompt(&a, HB_STREAM, err, sizeof err);
+  } else if (paged_op(K) >= 0) {
+    const int op = paged_op(K);
+    ThvmPagedArgs a;
+    NEED(paged_parse(&sp, op, &a) || paged_args(&c, op, &a));
+    const u64 kvb = (u64)a.n * 2 * a.Hkv, held = pg_row_bytes(a.hd, a.bits);
+    bytes = op == PG_APPEND ? ((u64)a.n * 2 * a.H + kvb) * a.hd * 2 + kvb * held
+          : op == PG_READ ? kvb * (held + a.hd * 2) : 0;     /* (attention: live-length dependent) */
+    if (check_only) return 0;
+    if (prof) hb_kprof_begin(K, &e0, &e1);
+    rc = op == PG_APPEND ? thvm_k_kv_append(&a, HB_STREAM, err, sizeof err)
+       : op == PG_READ ? thvm_k_kv_read(&a, HB_STREAM, err, sizeof err)
+                       : thvm_k_attn_paged(&a, HB_STREAM, err, sizeof err);
   } else if (strcmp(K, "mla_prep") == 0 || strcmp(K, "mla_attn") == 0) {
     ThvmMlaArgs a;
     memset(&a, 0, sizeof a);

@@ -301,6 +301,40 @@ int thvm_k_moe_down(const ThvmMoeArgs *a, hipStream_t s, char *err, int errlen);
  * H, Hkv, hd, max_seq, qdt, cdt, odt, scale and T. */
 int thvm_k_attn_prompt(const ThvmAttnArgs *a, hipStream_t s, char *err, int errlen);
 
+/* A paged cache and the calls on it.  n rows (new positions) of b sequences:
+ * sequence s has the rows [rows[s], rows[s+1]) of the call (rows NULL: n / b
+ * each), the last ones of its len[s] cache rows, so row i of them is position
+ * len[s] - count + i.  A pool holds npages pages of [Hkv][page] rows of one
+ * head: page x hd 16-bit values, or with bits = 4 page x hd / 2 bytes of e2m1
+ * codes (value 2i in the low nibble of byte i) and then page x hd / 32 bytes of
+ * e8m0 scales, one per 32 values.  table [b][maxpages] names a sequence's
+ * pages; an id outside [0, npages) is no page.
+ * All of rows, len and table are read on the device: values outside their
+ * ranges are never followed (a position with no page is not stored, not seen
+ * and read as zeros; rows of no sequence are left as they were). */
+typedef struct ThvmPagedArgs {
+  void *q;                 /* append: out [n][H][hd]; attn: in                */
+  void *out;               /* attn: [n][H][hd]                                */
+  void *kpages, *vpages;
+  const void *x;           /* append: [n][ldx], heads q, k, v of hd values    */
+  void *k, *v;             /* read: [n][Hkv][hd]                              */
+  const int32_t *table, *len, *rows;
+  const float *gq, *gk;    /* append, norm: [hd] gains                        */
+  const float *cos_t, *sin_t;   /* append, rope: [maxpages * page][hd / 2]    */
+  float *ws;               /* attn: thvm_k_attn_paged_ws bytes                */
+  uint32_t n, b, H, Hkv, hd, page, maxpages, npages, dt, bits;
+  uint32_t ragged;         /* rows is given                                   */
+  uint32_t rope;           /* 0 none, 1 pairs (2j, 2j+1), 2 pairs (j, j+hd/2) */
+  uint32_t norm, ldx;      /* RMS norm of every q and k head; row stride of x */
+  uint32_t t;              /* attn: most rows of a sequence (the caller's word:
+                            * a sequence with more is left out)              */
+  float eps, scale;
+} ThvmPagedArgs;
+int thvm_k_kv_append(const ThvmPagedArgs *a, hipStream_t s, char *err, int errlen);
+int thvm_k_kv_read(const ThvmPagedArgs *a, hipStream_t s, char *err, int errlen);
+int thvm_k_attn_paged(const ThvmPagedArgs *a, hipStream_t s, char *err, int errlen);
+uint64_t thvm_k_attn_paged_ws(const ThvmPagedArgs *a);
+
 /* Embedding gather: x[b][i] = emb[tok[b]][i] (+ pos[L-1][i] when pos != NULL;
  * with seq > 0 pos[L-1 + b % seq][i]: seq positions of each sequence), tok
  * int32 [B]; out of range ids read a zero row. */
