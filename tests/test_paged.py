@@ -65,7 +65,7 @@ def test_workspace_needs_no_device(lib):
     (dict(n=5), "divide"), (dict(ragged=2), "ragged"), (dict(maxpages=0), "positions"),
     (dict(maxpages=(1 << 26) + 1), "positions"), (dict(npages=0), "positions"), (dict(npages=1 << 31), "positions"),
     (dict(hkv=0), "hkv"), (dict(hkv=2000, h=2000), "hkv"), (dict(h=0), "multiple"), (dict(h=7), "multiple"),
-    (dict(h=2048, hkv=2), "multiple"), (dict(n=1 << 22, h=64), "heads"), (dict(t=0), "t=0"), (dict(t=1), "t=1"),
+    (dict(h=2048, hkv=2), "multiple"), (dict(n=1 << 22, h=64), "heads"), (dict(n=4096, b=4096, hkv=256, h=256), "2.19"), (dict(t=0), "t=0"), (dict(t=1), "t=1"),
     (dict(scale=float("inf")), "scale"), (dict(scale=float("nan")), "scale")])
 def test_attn_paged_specs_refused(lib, bad, word, monkeypatch):
     monkeypatch.setenv("THVM_HIP_QUIET", "1")

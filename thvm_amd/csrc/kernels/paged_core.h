@@ -57,3 +57,93 @@ __device__ __forceinline__ uint32_t fp4x2(uint32_t w, float scale) {
   return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, SEL));
 }
 __device__ __forceinline__ float e8m0_f(uint32_t byte) { return __uint_as_float(byte << 23); }
+
+// ---- units of work -----------------------------------------------------------
+// A kernel takes the sequences whose columns (rows x the G query heads of a kv
+// head) number more than lo and at most hi, ct columns a tile, and splits each
+// tile's cache rows into chunks of c steps of 64 rows.  Lengths are known on the
+// device only and differ, so c is chosen there, by every wave for itself and from
+// the same numbers: the smallest of a few tries between all steps / units and all
+// steps / (units - tiles) with which the chunks number at most `units`.  The last
+// try always does (a tile adds one chunk at most to its share); the host launches
+// units >= 2 x tiles, so c never passes the mean length of the tiles: long
+// sequences are split, short ones are not, and the blocks are of one size.
+struct PgPlan { uint32_t lo, hi, ct, units, cmin; };
+struct PgUnit { PgSeq q; uint32_t s, tile, chunk, nchunk, c, first; };
+
+__device__ __forceinline__ float wave_scan(float v) {           // inclusive, lane order
+  v += dpp_f<0x111>(v);
+  v += dpp_f<0x112>(v);
+  v += dpp_f<0x114>(v);
+  v += dpp_f<0x118>(v);
+  v += dpp_f<0x142, 0xa>(v);
+  v += dpp_f<0x143, 0xc>(v);
+  return v;
+}
+
+// unit u's tile and chunk, or (tiles_only) tile u's first unit; false: none.
+// Counts stay below 2^24 (2^25 heads / ct), exact in f32; the steps' sum need not
+// be.
+__device__ __forceinline__ bool pg_unit(const ThvmPagedArgs &a, const PgPlan &p, uint32_t u, bool tiles_only, PgUnit &o) {
+  const uint32_t lane = lane_id(), G = a.H / a.Hkv;
+  const int32_t cap = (int32_t)(a.maxpages * a.page);
+  // a lane's sequence of each 64: its tiles and steps (the first 64 kept)
+  auto load = [&](uint32_t s0, PgSeq &q, float &tiles, float &steps) {
+    const uint32_t s = s0 + lane;
+    tiles = steps = 0.0f;
+    if (s < a.b) {
+      q = pg_seq(&a, s);
+      const uint32_t rows = (uint32_t)(q.r1 - q.r0), cols = rows * G;
+      if (rows <= a.t && cols > p.lo && cols <= p.hi) tiles = (float)((cols + p.ct - 1) / p.ct);
+      steps = (float)max((min(q.len, cap) + 63) / 64, 1);
+    }
+  };
+  PgSeq q0 = {0, 0, 0}, q;
+  float t0, l0, tl, st;
+  load(0, q0, t0, l0);
+  auto each = [&](auto f) {
+    f(0u, q0, t0, l0);
+    for (uint32_t s0 = 64; s0 < a.b; s0 += 64) {
+      load(s0, q, tl, st);
+      f(s0, q, tl, st);
+    }
+  };
+  float total = 0.0f, tiles = 0.0f;
+  each([&](uint32_t, const PgSeq &, float t, float l) { total += wave_sum(t * l); tiles += wave_sum(t); });
+  if (tiles == 0.0f) return false;
+  const float units = (float)p.units;
+  const uint32_t c1 = max(p.cmin, (uint32_t)(total / units)), c2 = max(c1, (uint32_t)(total * 1.0001f / (units - tiles)) + 1);
+  uint32_t c = c1;
+  for (int k = 1;; k++) {
+    if (k > 4) { c = c2; break; }
+    float n = 0.0f;
+    each([&](uint32_t, const PgSeq &, float t, float l) { n += wave_sum(t * (float)(((uint32_t)l + c - 1) / c)); });
+    if (n <= units) break;
+    c = c1 + (uint32_t)((uint64_t)(c2 - c1) * k / 4);
+  }
+  o.c = c;
+  float before = 0.0f, tbefore = 0.0f;
+  bool found = false;
+  each([&](uint32_t s0, const PgSeq &q, float t, float l) {
+    if (found) return;
+    const float per = (float)(((uint32_t)l + c - 1) / c), n = t * per, sc = wave_scan(n), tc = wave_scan(t);
+    const uint64_t hit = __builtin_amdgcn_ballot_w64((tiles_only ? tbefore + tc : before + sc) > (float)u);
+    if (hit) {
+      const int w = __builtin_ctzll(hit);
+      auto at = [&](float v) { return (uint32_t)__int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), w)); };
+      found = true;
+      o.s = s0 + w;
+      o.q.r0 = __builtin_amdgcn_readlane(q.r0, w);
+      o.q.r1 = __builtin_amdgcn_readlane(q.r1, w);
+      o.q.len = __builtin_amdgcn_readlane(q.len, w);
+      o.nchunk = at(per);
+      const uint32_t first = at(before + sc - n), tfirst = at(tbefore + tc - t);
+      o.tile = tiles_only ? u - tfirst : (u - first) / o.nchunk;
+      o.chunk = tiles_only ? 0 : (u - first) % o.nchunk;
+      o.first = first + o.tile * o.nchunk;
+    }
+    before += wave_sum(n);
+    tbefore += wave_sum(t);
+  });
+  return found;
+}

@@ -36,7 +36,8 @@ static inline int pg_check(const ThvmPagedArgs *a, int op, char *err, int errlen
   if (a->Hkv == 0 || a->Hkv > 1024) PG_REFUSE("hkv from 1 to 1024 (hkv=%u)", a->Hkv);
   if (op != PG_READ && (a->H == 0 || a->H > 1024 || a->H % a->Hkv))
     PG_REFUSE("h from 1 to 1024, a multiple of hkv (h=%u hkv=%u)", a->H, a->Hkv);
-  /* (a wave per 4 heads or more: grids stay below 2^32 threads) */
+  /* (grids stay below 2^32 threads) */
+  if ((uint64_t)a->b * a->Hkv > (1u << 19)) PG_REFUSE("b x hkv of more than 2^19 (b=%u hkv=%u)", a->b, a->Hkv);
   if ((uint64_t)a->n * (op == PG_READ ? 2 * a->Hkv : a->H + 2 * a->Hkv) > (1u << 25))
     PG_REFUSE("more than 2^25 heads in all rows (n=%u)", a->n);
   if (op == PG_APPEND) {
