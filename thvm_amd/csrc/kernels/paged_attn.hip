@@ -2,88 +2,14 @@
 //
 // out = sum_j softmax_j(scale q.k_j) v_j over the cache rows j <= p that have a
 // page, for every row (position p of its sequence) and head; no such row: zeros.
-// A wave takes one (row, head): 64 cache rows at a time, a lane's own row for the
-// scores, a lane's own columns for the weighted sum.  Softmax statistics and sums
+// The rows and the query heads of a kv head are the columns of its products.
+// Sequences of few columns (single tokens, speculative rows) go to k_paged_split
+// here, the others to k_paged_tile (paged_prompt.hip); either splits long contexts
+// into chunks whose partial sums k_paged_merge adds.  Softmax statistics and sums
 // are f32.
 #include "paged_core.h"
 
-#define PA_WAVES 4
 #define LOG2E 1.4426950408889634f
-
-template <int HD, int XT, int BITS>
-__global__ __launch_bounds__(PA_WAVES * 64) void k_paged_rows(ThvmPagedArgs a, PgPlan pl) {
-  typedef PgT<XT> P;
-  constexpr int NC = HD / 64;                             // columns of a lane
-  __shared__ float qs[PA_WAVES][HD];
-  const uint32_t wv = threadIdx.x >> 6, lane = lane_id();
-  const uint32_t unit = __builtin_amdgcn_readfirstlane(blockIdx.x * PA_WAVES + wv), row = unit / a.H, h = unit % a.H;
-  if (row >= a.n) return;
-  const uint32_t s = pg_seq_of(a, row);
-  if (s >= a.b) return;
-  const PgSeq sq = pg_seq(&a, s);
-  if ((int32_t)row < sq.r0 || (int32_t)row >= sq.r1 || (uint32_t)(sq.r1 - sq.r0) > a.t) return;
-  if ((uint32_t)(sq.r1 - sq.r0) * (a.H / a.Hkv) <= pl.lo) return;
-  const int32_t pos = sq.len - (sq.r1 - (int32_t)row);
-  const int32_t lim = min(pos + 1, (int32_t)(a.maxpages * a.page));
-  const uint32_t kvh = h / (a.H / a.Hkv);
-  const uint16_t *q = (const uint16_t *)a.q + ((uint64_t)row * a.H + h) * HD;
-  for (uint32_t d = lane; d < HD; d += 64) qs[wv][d] = P::lo(q[d]) * a.scale * LOG2E;
-  __builtin_amdgcn_wave_barrier();                        // a wave's own LDS accesses stay in order
-  float m = -INFINITY, l = 0.0f, acc[NC] = {};
-  for (int32_t j0 = 0; j0 < lim; j0 += 64) {
-    const int32_t j = j0 + (int32_t)lane;
-    const int32_t id = j < lim ? pg_page(&a, s, j) : -1;
-    const uint64_t blk = id >= 0 ? pg_block(&a, id, kvh) : 0;
-    const uint32_t slot = (uint32_t)j & (a.page - 1);
-    float sc = -INFINITY;
-    if (id >= 0) {
-      sc = 0.0f;
-      const char *kb = (const char *)a.kpages + blk;
-      for (int d = 0; d < HD; d += 8) {
-        uint4 w;
-        if (BITS == 16) {
-          w = ld16(kb + (slot * HD + d) * 2);
-        } else {
-          const uint32_t c = *(const uint32_t *)(kb + slot * (HD / 2) + d / 2);
-          const float f = e8m0_f((uint8_t)kb[a.page * (HD / 2) + slot * (HD / 32) + d / 32]);
-          w = make_uint4(fp4x2<XT, 0>(c, f), fp4x2<XT, 1>(c, f), fp4x2<XT, 2>(c, f), fp4x2<XT, 3>(c, f));
-        }
-        const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-        for (int i = 0; i < 4; i++) sc += P::lo(ww[i]) * qs[wv][d + 2 * i] + P::hi(ww[i]) * qs[wv][d + 2 * i + 1];
-      }
-    }
-    const float mn = fmaxf(m, wave_max(sc));
-    const float f = m == -INFINITY ? 0.0f : exp2f(m - mn), p = id < 0 ? 0.0f : exp2f(sc - mn);
-    l = l * f + wave_sum(p);
-    m = mn;
-#pragma unroll
-    for (int c = 0; c < NC; c++) acc[c] *= f;
-    for (int r = 0; r < 64; r++) {
-      const int32_t rid = __builtin_amdgcn_readlane(id, r);
-      if (rid < 0) continue;
-      const float pr = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(p), r));
-      const char *vb = (const char *)a.vpages + pg_block(&a, rid, kvh);
-      const uint32_t rs = (uint32_t)(j0 + r) & (a.page - 1);
-#pragma unroll
-      for (int c = 0; c < NC; c++) {
-        const uint32_t d = lane + 64 * c;
-        float x;
-        if (BITS == 16) {
-          x = P::lo(((const uint16_t *)vb)[rs * HD + d]);
-        } else {
-          const uint32_t two = fp4x2<XT, 0>((uint8_t)vb[rs * (HD / 2) + d / 2],
-                                            e8m0_f((uint8_t)vb[a.page * (HD / 2) + rs * (HD / 32) + d / 32]));
-          x = d & 1 ? P::hi(two) : P::lo(two);
-        }
-        acc[c] += pr * x;
-      }
-    }
-  }
-  uint16_t *o = (uint16_t *)a.out + ((uint64_t)row * a.H + h) * HD;
-#pragma unroll
-  for (int c = 0; c < NC; c++) o[lane + 64 * c] = (uint16_t)P::pk(l != 0.0f ? acc[c] / l : 0.0f, 0.0f);
-}
 
 // ---- a few columns: the split -------------------------------------------------
 // k_paged_split: a unit is one tile of at most 16 columns (rows x query heads of
@@ -105,8 +31,6 @@ __global__ __launch_bounds__(PA_WAVES * 64) void k_paged_rows(ThvmPagedArgs a, P
 #define PS_WAVES 4
 #define PS_THREADS (PS_WAVES * 64)
 
-template <int XT> struct PsFin { static constexpr uint32_t EXP = XT == GX_BF16 ? 0x7f80u : 0x7c00u; };
-
 // cached bytes in registers on their way to MFMA operands
 template <int HD, int BITS> struct PsRegs;
 template <> struct PsRegs<128, 16> { uint4 k[4][4]; uint4 v[4][4]; };
@@ -118,7 +42,8 @@ template <int HD, int XT, int BITS, int CG>
 __global__ __launch_bounds__(PS_THREADS, 2) void k_paged_split(ThvmPagedArgs a, PgPlan pl) {
   typedef PgT<XT> P;
   constexpr int EC = HD / 16, KS = HD / 32, NG = 16 / CG, NS = 4 / NG, RB = BITS == 16 ? HD * 2 : HD / 2;
-  constexpr uint32_t EXP = PsFin<XT>::EXP;
+  constexpr uint32_t EXP = XT == GX_BF16 ? 0x7f80u : 0x7c00u;
+  constexpr float PSH = XT == GX_BF16 ? 0.0f : 14.0f;      // keeps small p off fp16's subnormals; cancels in acc / l
   __shared__ __align__(16) float wacc[PS_WAVES][16][HD + 4];
   __shared__ float wm[PS_WAVES][16], wl[PS_WAVES][16];
   const uint32_t kvh = blockIdx.x % a.Hkv, un = blockIdx.x / a.Hkv, G = a.H / a.Hkv;
@@ -264,7 +189,7 @@ __global__ __launch_bounds__(PS_THREADS, 2) void k_paged_split(ThvmPagedArgs a, 
 #pragma unroll
     for (int s = 0; s < NS; s++) {
 #pragma unroll
-      for (int i = 0; i < 4; i++) p[s][i] = p[s][i] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(p[s][i] - mn);
+      for (int i = 0; i < 4; i++) p[s][i] = p[s][i] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(p[s][i] - (mn - PSH));
       ls += (p[s][0] + p[s][1]) + (p[s][2] + p[s][3]);
       pk[s][0] = P::pk(p[s][0], p[s][1]);
       pk[s][1] = P::pk(p[s][2], p[s][3]);
@@ -436,113 +361,125 @@ __global__ __launch_bounds__(PS_THREADS, 2) void k_paged_split(ThvmPagedArgs a, 
   }
 }
 
-// k_paged_merge: the chunks of one column, their partials (sum, m, l) in chunk
-// order: 8 groups of 32 lanes take every eighth chunk, then meet in LDS.
-template <int HD, int XT, int CT>
+// k_paged_merge: the chunks of a column, their partials (sum, m, l) in a fixed
+// order.  HD / 4 lanes take a chunk; NP such groups take every NP-th chunk of one
+// column and meet in LDS, the block's other groups have other columns.
+template <int HD, int XT, int CT, int NP>
 __global__ __launch_bounds__(256) void k_paged_merge(ThvmPagedArgs a, PgPlan pl) {
   typedef PgT<XT> P;
-  constexpr int LN = HD / 4, NP = 256 / LN;                // lanes a chunk, chunks side by side
-  __shared__ float4 ls[NP][LN];
-  __shared__ float lm[NP], ll[NP];
-  const uint32_t c = blockIdx.x % CT, kvh = blockIdx.x / CT % a.Hkv, G = a.H / a.Hkv;
+  constexpr int LN = HD / 4, NG = 256 / LN, CB = NG / NP;  // lanes a chunk, groups, columns a block
+  __shared__ float4 ls[NG][LN];
+  __shared__ float lm[NG], ll[NG];
+  const uint32_t g = threadIdx.x / LN, x = threadIdx.x % LN, part = g % NP;
+  const uint32_t c = blockIdx.x % (CT / CB) * CB + g / NP, kvh = blockIdx.x / (CT / CB) % a.Hkv, G = a.H / a.Hkv;
   PgUnit u;
-  if (!pg_unit(a, pl, blockIdx.x / CT / a.Hkv, true, u) || u.nchunk == 1) return;
+  if (!pg_unit(a, pl, blockIdx.x / (CT / CB) / a.Hkv, true, u) || u.nchunk == 1) return;
   const uint32_t cc = u.tile * pl.ct + c;
-  if ((int32_t)(cc / G) >= u.q.r1 - u.q.r0) return;
-  const uint32_t part = threadIdx.x / LN, x = threadIdx.x % LN;
+  const bool live = (int32_t)(cc / G) < u.q.r1 - u.q.r0;
   const float *pp = a.ws + (((uint64_t)kvh * pl.units + u.first) * CT + c) * (HD + 4);
   const uint64_t st = (uint64_t)CT * (HD + 4);
   float m = -INFINITY, l = 0.0f;
   float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (uint32_t k = part; k < u.nchunk; k += NP) {
+  for (uint32_t k = part; live && k < u.nchunk; k += NP) {
     const float4 w = *(const float4 *)(pp + k * st + 4 * x);
     const float2 ml = *(const float2 *)(pp + k * st + HD);
     const float mn = fmaxf(m, ml.x), f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn),
-                g = ml.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml.x - mn);
-    v.x = v.x * f + w.x * g;
-    v.y = v.y * f + w.y * g;
-    v.z = v.z * f + w.z * g;
-    v.w = v.w * f + w.w * g;
-    l = l * f + ml.y * g;
+                e = ml.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml.x - mn);
+    v.x = v.x * f + w.x * e;
+    v.y = v.y * f + w.y * e;
+    v.z = v.z * f + w.z * e;
+    v.w = v.w * f + w.w * e;
+    l = l * f + ml.y * e;
     m = mn;
   }
-  ls[part][x] = v;
-  if (x == 0) { lm[part] = m; ll[part] = l; }
-  __syncthreads();
-  if (threadIdx.x >= LN) return;
-  float M = -INFINITY;
+  if (NP > 1) {
+    ls[g][x] = v;
+    if (x == 0) { lm[g] = m; ll[g] = l; }
+    __syncthreads();
+    if (part) return;
+    float M = -INFINITY;
 #pragma unroll
-  for (int k = 0; k < NP; k++) M = fmaxf(M, lm[k]);
-  l = 0.0f;
-  v = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int k = 0; k < NP; k++) M = fmaxf(M, lm[g + k]);
+    l = 0.0f;
+    v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-  for (int k = 0; k < NP; k++) {
-    const float f = lm[k] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(lm[k] - M);
-    v.x += ls[k][x].x * f;
-    v.y += ls[k][x].y * f;
-    v.z += ls[k][x].z * f;
-    v.w += ls[k][x].w * f;
-    l += ll[k] * f;
+    for (int k = 0; k < NP; k++) {
+      const float f = lm[g + k] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(lm[g + k] - M);
+      v.x += ls[g + k][x].x * f;
+      v.y += ls[g + k][x].y * f;
+      v.z += ls[g + k][x].z * f;
+      v.w += ls[g + k][x].w * f;
+      l += ll[g + k] * f;
+    }
   }
+  if (!live) return;
   const float inv = l != 0.0f ? 1.0f / l : 0.0f;
   *(uint2 *)((uint16_t *)a.out + ((uint64_t)(u.q.r0 + cc / G) * a.H + kvh * G + cc % G) * HD + 4 * x) =
       make_uint2(P::pk(v.x * inv, v.y * inv), P::pk(v.z * inv, v.w * inv));
 }
 
 // ---- which kernels a call takes ------------------------------------------------
-struct PaRule { bool few, many; uint32_t cg; PgPlan few_pl; };
+// few: sequences of up to few.hi columns, cg of the MFMA's 16 columns used; many:
+// the others, chunks of them (split) where their tiles do not fill the chip.
+struct PaRule { bool few, many, split; uint32_t cg, few_tiles, many_tiles; PgPlan fpl, mpl; };
 static PaRule pa_rule(const ThvmPagedArgs *a) {
   PaRule r;
-  const uint32_t G = a->H / a->Hkv, t = a->t < a->n ? a->t : a->n;
+  const uint32_t G = a->H / a->Hkv, t = a->t < a->n ? a->t : a->n, fill = (512 + a->Hkv - 1) / a->Hkv;
   const uint64_t most = (uint64_t)t * G;                   // columns of the longest sequence
   const uint32_t cols = most <= 16 ? (uint32_t)most : G;
   r.cg = cols <= 4 ? 4 : cols <= 8 ? 8 : 16;
   const uint32_t hi = most <= 16 || r.cg > G ? r.cg : G;
   r.many = most > hi;
   r.few = !r.many || a->ragged;
-  const uint32_t tiles = a->b * ((hi + 15) / 16), want = (512 + a->Hkv - 1) / a->Hkv;
-  r.few_pl = PgPlan{0, hi, 16, want > 2 * tiles ? want : 2 * tiles, 1};
+  r.few_tiles = a->b * ((hi + 15) / 16);
+  r.fpl = PgPlan{0, hi, 16, fill > 2 * r.few_tiles ? fill : 2 * r.few_tiles, 1};
+  const uint32_t whole = (uint32_t)((uint64_t)a->n * G / PP_COLS);
+  r.many_tiles = whole + a->b;
+  r.split = (uint64_t)whole * a->Hkv < 512;
+  r.mpl = PgPlan{r.few ? hi : 0, 0xffffffffu, PP_COLS, r.many_tiles + 1, 1u << 25};
+  if (r.split) {
+    r.mpl.units = fill > 2 * r.many_tiles ? fill : 2 * r.many_tiles;
+    r.mpl.cmin = 4;
+  }
   return r;
 }
 
 extern "C" uint64_t thvm_k_attn_paged_ws(const ThvmPagedArgs *a) {
   const PaRule r = pa_rule(a);
-  return r.few ? (uint64_t)a->Hkv * r.few_pl.units * r.cg * (a->hd + 4) * 4 : 16;
+  const uint64_t rec = (uint64_t)a->Hkv * (a->hd + 4) * 4, f = r.few ? rec * r.fpl.units * r.cg : 0,
+                 m = r.many && r.split ? rec * r.mpl.units * PP_COLS : 0;
+  return f > m ? f : m > 16 ? m : 16;
 }
 
-typedef void (*paged_fn)(ThvmPagedArgs, PgPlan);
 template <int HD, int XT, int BITS>
 static paged_fn pa_split(uint32_t cg) {
   return cg == 4 ? k_paged_split<HD, XT, BITS, 4> : cg == 8 ? k_paged_split<HD, XT, BITS, 8> : k_paged_split<HD, XT, BITS, 16>;
 }
+struct PaKernels { paged_fn split, merge, tmerge; };
 template <int HD, int XT>
-static paged_fn pa_merge(uint32_t cg) {
-  return cg == 4 ? k_paged_merge<HD, XT, 4> : cg == 8 ? k_paged_merge<HD, XT, 8> : k_paged_merge<HD, XT, 16>;
-}
-template <int HD, int XT>
-static void pa_pick(const ThvmPagedArgs *a, uint32_t cg, paged_fn *split, paged_fn *merge, paged_fn *rows) {
-  *split = a->bits == 16 ? pa_split<HD, XT, 16>(cg) : pa_split<HD, XT, 4>(cg);
-  *merge = pa_merge<HD, XT>(cg);
-  *rows = a->bits == 16 ? k_paged_rows<HD, XT, 16> : k_paged_rows<HD, XT, 4>;
+static PaKernels pa_pick(const ThvmPagedArgs *a, uint32_t cg) {
+  constexpr int NG = 1024 / HD;                            // one column a block
+  return PaKernels{a->bits == 16 ? pa_split<HD, XT, 16>(cg) : pa_split<HD, XT, 4>(cg),
+                   cg == 4 ? k_paged_merge<HD, XT, 4, NG> : cg == 8 ? k_paged_merge<HD, XT, 8, NG> : k_paged_merge<HD, XT, 16, NG>,
+                   k_paged_merge<HD, XT, PP_COLS, 2>};
 }
 
 extern "C" int thvm_k_attn_paged(const ThvmPagedArgs *a, hipStream_t s, char *err, int errlen) {
   if (pg_check(a, PG_ATTN, err, errlen)) return -1;
   const PaRule r = pa_rule(a);
   const int bf = a->dt == THVM_DT_BF16;
-  paged_fn split, merge, rows;
-  if (a->hd == 128) { if (bf) pa_pick<128, GX_BF16>(a, r.cg, &split, &merge, &rows); else pa_pick<128, GX_F16>(a, r.cg, &split, &merge, &rows); }
-  else { if (bf) pa_pick<64, GX_BF16>(a, r.cg, &split, &merge, &rows); else pa_pick<64, GX_F16>(a, r.cg, &split, &merge, &rows); }
+  const PaKernels k = a->hd == 128 ? (bf ? pa_pick<128, GX_BF16>(a, r.cg) : pa_pick<128, GX_F16>(a, r.cg))
+                                   : (bf ? pa_pick<64, GX_BF16>(a, r.cg) : pa_pick<64, GX_F16>(a, r.cg));
   if (r.few) {
-    const uint32_t tiles = a->b * ((r.few_pl.hi + 15) / 16);
-    thvm_launch(true, false, split, dim3(a->Hkv * r.few_pl.units), dim3(PS_THREADS), 0, s, *a, r.few_pl);
-    thvm_launch(false, !r.many, merge, dim3(a->Hkv * r.cg * tiles), dim3(256), 0, s, *a, r.few_pl);
+    thvm_launch(true, false, k.split, dim3(a->Hkv * r.fpl.units), dim3(PS_THREADS), 0, s, *a, r.fpl);
+    thvm_launch(false, !r.many, k.merge, dim3(a->Hkv * r.cg * r.few_tiles), dim3(256), 0, s, *a, r.fpl);
   }
   if (r.many) {
-    PgPlan pl = r.few_pl;
-    pl.lo = pl.hi;
-    const uint64_t units = (uint64_t)a->n * a->H;
-    thvm_launch(!r.few, true, rows, dim3((uint32_t)((units + PA_WAVES - 1) / PA_WAVES)), dim3(PA_WAVES * 64), 0, s, *a, pl);
+    thvm_launch(!r.few, !r.split, pp_tile_pick(a), dim3(a->Hkv * r.mpl.units), dim3(PP_THREADS), 0, s, *a, r.mpl);
+    if (r.split) {
+      const uint32_t cb = 256 / (a->hd / 4) / 2;           // columns a block
+      thvm_launch(false, true, k.tmerge, dim3(a->Hkv * (PP_COLS / cb) * r.many_tiles), dim3(256), 0, s, *a, r.mpl);
+    }
   }
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) { snprintf(err, errlen, "attn_paged launch: %s", hipGetErrorString(e)); return -1; }

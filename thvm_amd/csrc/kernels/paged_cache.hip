@@ -143,13 +143,13 @@ __global__ __launch_bounds__(PC_THREADS) void k_kv_read(ThvmPagedArgs a) {
   *(uint4 *)((uint16_t *)(hv < a.Hkv ? a.k : a.v) + ((uint64_t)row * a.Hkv + kvh) * HD + d0) = w;
 }
 
-typedef void (*paged_fn)(ThvmPagedArgs);
+typedef void (*pc_fn)(ThvmPagedArgs);
 #define PC_PICK(K) (a->hd == 128 ? (bf ? (a->bits == 16 ? K<128, GX_BF16, 16> : K<128, GX_BF16, 4>)          \
                                        : (a->bits == 16 ? K<128, GX_F16, 16> : K<128, GX_F16, 4>))          \
                                  : (bf ? (a->bits == 16 ? K<64, GX_BF16, 16> : K<64, GX_BF16, 4>)            \
                                        : (a->bits == 16 ? K<64, GX_F16, 16> : K<64, GX_F16, 4>)))
 
-static int pc_launch(paged_fn f, const ThvmPagedArgs *a, uint32_t heads, const char *who, hipStream_t s, char *err,
+static int pc_launch(pc_fn f, const ThvmPagedArgs *a, uint32_t heads, const char *who, hipStream_t s, char *err,
                      int errlen) {
   const uint32_t vpw = 64 / (a->hd / 8);
   const uint64_t waves = (uint64_t)a->n * ((heads + vpw - 1) / vpw);

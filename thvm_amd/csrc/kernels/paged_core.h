@@ -147,3 +147,10 @@ __device__ __forceinline__ bool pg_unit(const ThvmPagedArgs &a, const PgPlan &p,
   });
   return found;
 }
+
+typedef void (*paged_fn)(ThvmPagedArgs, PgPlan);
+// the kernel of many columns (paged_prompt.hip), PP_COLS a block
+#define PP_WAVES 4
+#define PP_THREADS (PP_WAVES * 64)
+#define PP_COLS (PP_WAVES * 32)
+paged_fn pp_tile_pick(const ThvmPagedArgs *a);
