@@ -254,6 +254,19 @@ def test_attn_paged_later_positions_that_are_not_finite(hip, bits, bad, seqs):
             assert near(got[row].astype(np.float64), want, tol, DT_BF16), row
 
 
+@pytest.mark.parametrize("scale", [0.0, -0.125, 3.0, 1e-38, -2e4])
+@pytest.mark.parametrize("seqs", [[(1, 50), (1, 9)], [(40, 75), (33, 33)]])
+def test_attn_paged_scales(hip, scale, seqs):
+    """Any finite scale: none (the mean of the rows), negative, and so large that one row takes all."""
+    say(f"case: attn_paged scale={scale} {seqs}")
+    P = Paged(seqs, DT_BF16, 16, 4, 2, 64, 16)
+    q = O.encode((0.01 * P.rng.standard_normal((P.n, 4, 64)) if abs(scale) > 10 else
+                  P.rng.standard_normal((P.n, 4, 64))).astype(np.float32), DT_BF16)
+    kpool, vpool = P.filled(), P.filled()
+    scale = np.float32(scale)
+    check_attn(P, q, kpool, vpool, attn(hip, P, q, kpool, vpool, scale), scale)
+
+
 def test_attn_paged_t_leaves_longer_sequences_out(hip):
     say("case: attn_paged t")
     P = Paged([(1, 40), (6, 40), (2, 9)], DT_BF16, 16, 4, 2, 64, 16)

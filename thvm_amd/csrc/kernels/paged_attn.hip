@@ -25,8 +25,9 @@
 //   A wave's four tiles are 64 rows apart (wave w has rows 16 w .. of each 64), so a
 //   chunk of 64 rows still feeds all four waves, and every tile lies inside a page.
 // Over 4 bits a lane's K bytes are 32 (hd 64: 16) consecutive values, one scale;
-// the q operand is ordered to match.  p is rounded once to the 16-bit type for the
-// product (the cached values' own precision); its sum, like all else, is f32.
+// the q operand is ordered to match.  p enters the product as a pair of 16-bit terms
+// (hi and what it leaves: 16 bits of p in bf16, 22 in fp16), which costs nothing where
+// the cache's bytes are the bound; its sum, like all else, is f32.
 // Bound by the cache's bytes.
 #define PS_WAVES 4
 #define PS_THREADS (PS_WAVES * 64)
@@ -185,14 +186,17 @@ __global__ __launch_bounds__(PS_THREADS, 2) void k_paged_split(ThvmPagedArgs a, 
     mx = fmaxf(mx, xor32_f(mx));
     const float mn = fmaxf(m, mx), f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
     float ls = 0.0f;
-    uint32_t pk[NS][2];
+    uint32_t pk[NS][2], pl2[NS][2];
 #pragma unroll
     for (int s = 0; s < NS; s++) {
 #pragma unroll
       for (int i = 0; i < 4; i++) p[s][i] = p[s][i] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(p[s][i] - (mn - PSH));
       ls += (p[s][0] + p[s][1]) + (p[s][2] + p[s][3]);
-      pk[s][0] = P::pk(p[s][0], p[s][1]);
-      pk[s][1] = P::pk(p[s][2], p[s][3]);
+#pragma unroll
+      for (int i = 0; i < 2; i++) {                        // hi + lo, the differences exact
+        pk[s][i] = P::pk(p[s][2 * i], p[s][2 * i + 1]);
+        pl2[s][i] = P::pk(p[s][2 * i] - P::lo(pk[s][i]), p[s][2 * i + 1] - P::hi(pk[s][i]));
+      }
     }
     l = l * f + ls;
     m = mn;
@@ -266,14 +270,10 @@ __global__ __launch_bounds__(PS_THREADS, 2) void k_paged_split(ThvmPagedArgs a, 
     }
 #pragma unroll
     for (int h = 0; h < 2; h++) {                          // tiles 2h and 2h + 1
-      uint4 B;
-      {
-        const int s0 = (2 * h) / NG, g0 = (2 * h) % NG, s1 = (2 * h + 1) / NG, g1 = (2 * h + 1) % NG;
-        B.x = NG == 1 || lc / CG == g0 ? pk[s0][0] : 0u;
-        B.y = NG == 1 || lc / CG == g0 ? pk[s0][1] : 0u;
-        B.z = NG == 1 || lc / CG == g1 ? pk[s1][0] : 0u;
-        B.w = NG == 1 || lc / CG == g1 ? pk[s1][1] : 0u;
-      }
+      const int s0 = (2 * h) / NG, g0 = (2 * h) % NG, s1 = (2 * h + 1) / NG, g1 = (2 * h + 1) % NG;
+      const bool in0 = NG == 1 || lc / CG == g0, in1 = NG == 1 || lc / CG == g1;
+      const uint4 B = make_uint4(in0 ? pk[s0][0] : 0u, in0 ? pk[s0][1] : 0u, in1 ? pk[s1][0] : 0u, in1 ? pk[s1][1] : 0u);
+      const uint4 B2 = make_uint4(in0 ? pl2[s0][0] : 0u, in0 ? pl2[s0][1] : 0u, in1 ? pl2[s1][0] : 0u, in1 ? pl2[s1][1] : 0u);
 #pragma unroll
       for (int e = 0; e < EC; e++) {
         const uint32_t sel = (e & 1) ? 0x07060302u : 0x05040100u;
@@ -283,6 +283,7 @@ __global__ __launch_bounds__(PS_THREADS, 2) void k_paged_split(ThvmPagedArgs a, 
         A.z = __builtin_amdgcn_perm(w[2 * h + 1][1][e >> 1], w[2 * h + 1][0][e >> 1], sel);
         A.w = __builtin_amdgcn_perm(w[2 * h + 1][3][e >> 1], w[2 * h + 1][2][e >> 1], sel);
         acc[e] = mfma16<XT>(A, B, acc[e]);
+        acc[e] = mfma16<XT>(A, B2, acc[e]);
       }
     }
     if (fix) {                                             // wave-uniform
@@ -432,11 +433,11 @@ static PaRule pa_rule(const ThvmPagedArgs *a) {
   r.many = most > hi;
   r.few = !r.many || a->ragged;
   r.few_tiles = a->b * ((hi + 15) / 16);
-  r.fpl = PgPlan{0, hi, 16, fill > 2 * r.few_tiles ? fill : 2 * r.few_tiles, 1};
+  r.fpl = PgPlan{0, hi, 16, fill > 2 * r.few_tiles ? fill : 2 * r.few_tiles, 1, 0};
   const uint32_t whole = (uint32_t)((uint64_t)a->n * G / PP_COLS);
   r.many_tiles = whole + a->b;
   r.split = (uint64_t)whole * a->Hkv < 512;
-  r.mpl = PgPlan{r.few ? hi : 0, 0xffffffffu, PP_COLS, r.many_tiles + 1, 1u << 25};
+  r.mpl = PgPlan{r.few ? hi : 0, 0xffffffffu, PP_COLS, r.many_tiles + 1, 1u << 25, 1};
   if (r.split) {
     r.mpl.units = fill > 2 * r.many_tiles ? fill : 2 * r.many_tiles;
     r.mpl.cmin = 4;

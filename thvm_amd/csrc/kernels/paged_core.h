@@ -11,11 +11,20 @@ template <> struct PgT<GX_BF16> {
   static __device__ __forceinline__ float lo(uint32_t w) { return __uint_as_float(w << 16); }
   static __device__ __forceinline__ float hi(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
   static __device__ __forceinline__ uint32_t pk(float a, float b) { return pk_bf16(a, b); }
+  // c + both values of w, in f32
+  static __device__ __forceinline__ float sum2(uint32_t w, float c) {
+    typedef __bf16 b2_t __attribute__((ext_vector_type(2)));
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(b2_t, w), __builtin_bit_cast(b2_t, 0x3f803f80u), c, false);
+  }
 };
 template <> struct PgT<GX_F16> {
   static __device__ __forceinline__ float lo(uint32_t w) { return h2f((f16_t)(w & 0xffffu)); }
   static __device__ __forceinline__ float hi(uint32_t w) { return h2f((f16_t)(w >> 16)); }
   static __device__ __forceinline__ uint32_t pk(float a, float b) { return pk_f16(a, b); }
+  static __device__ __forceinline__ float sum2(uint32_t w, float c) {
+    typedef _Float16 h2_t __attribute__((ext_vector_type(2)));
+    return __builtin_amdgcn_fdot2(__builtin_bit_cast(h2_t, w), __builtin_bit_cast(h2_t, 0x3c003c00u), c, false);
+  }
 };
 
 // the sequence of row r, wave-uniform r: the one whose rows end first behind r
@@ -68,8 +77,8 @@ __device__ __forceinline__ float e8m0_f(uint32_t byte) { return __uint_as_float(
 // try always does (a tile adds one chunk at most to its share); the host launches
 // units >= 2 x tiles, so c never passes the mean length of the tiles: long
 // sequences are split, short ones are not, and the blocks are of one size.
-struct PgPlan { uint32_t lo, hi, ct, units, cmin; };
-struct PgUnit { PgSeq q; uint32_t s, tile, chunk, nchunk, c, first; };
+struct PgPlan { uint32_t lo, hi, ct, units, cmin, rev; };
+struct PgUnit { PgSeq q; uint32_t s, tile, chunk, nchunk, c, first, u; };
 
 __device__ __forceinline__ float wave_scan(float v) {           // inclusive, lane order
   v += dpp_f<0x111>(v);
@@ -122,6 +131,13 @@ __device__ __forceinline__ bool pg_unit(const ThvmPagedArgs &a, const PgPlan &p,
     c = c1 + (uint32_t)((uint64_t)(c2 - c1) * k / 4);
   }
   o.c = c;
+  if (p.rev && !tiles_only) {                                          // a block per unit: the last ones first
+    float n = 0.0f;
+    each([&](uint32_t, const PgSeq &, float t, float l) { n += wave_sum(t * (float)(((uint32_t)l + c - 1) / c)); });
+    if ((float)u >= n) return false;
+    u = (uint32_t)n - 1 - u;
+  }
+  o.u = u;
   float before = 0.0f, tbefore = 0.0f;
   bool found = false;
   each([&](uint32_t s0, const PgSeq &q, float t, float l) {

@@ -20,7 +20,7 @@
 // The running maximum moves only when a score passes it by 2^6 (the sums are f32
 // and p has room: up to 2^6 in bf16, 2^14 of fp16's 2^16 with p scaled by 2^8,
 // which keeps small p off fp16's subnormals); p is rounded once, to the 16-bit type
-// of the values it multiplies, and its sum is f32.
+// of the values it multiplies, and its sum, in f32, is that of the rounded ones.
 // Bound by the matrix and exponential units.
 #include "paged_core.h"
 
@@ -77,6 +77,15 @@ __global__ __launch_bounds__(PP_THREADS, 2) void k_paged_tile(ThvmPagedArgs a, P
   for (int ks = 0; ks < KS; ks++)
     qb[ks] = live ? ld16((const uint16_t *)a.q + ((uint64_t)(u.q.r0 + ri) * a.H + kvh * G + hg) * HD + 16 * ks + 8 * h)
                   : make_uint4(0, 0, 0, 0);
+  // scores are scaled inside the exponent, by a positive number: a negative scale's
+  // sign goes to q, and with a scale of zero (or too near for f32) q is zero
+  const bool none = fabsf(a.scale) < 1e-37f;
+  const float qs = none ? 1.0f : fabsf(a.scale) * LOG2E;
+  if (none || a.scale < 0.0f)
+#pragma unroll
+    for (int ks = 0; ks < KS; ks++)
+      qb[ks] = none ? make_uint4(0, 0, 0, 0)
+                    : make_uint4(qb[ks].x ^ 0x80008000u, qb[ks].y ^ 0x80008000u, qb[ks].z ^ 0x80008000u, qb[ks].w ^ 0x80008000u);
   const buf_t tb = buf_rsrc(a.table + (uint64_t)u.s * a.maxpages, a.maxpages * 4);
   const uint32_t lgp = __builtin_ctz(a.page), pm = a.page - 1, bb = pg_block_bytes(&a);
   const int nt = r1 > r0 ? (r1 - r0 + PP_STEP - 1) / PP_STEP : 0;
@@ -155,7 +164,6 @@ __global__ __launch_bounds__(PP_THREADS, 2) void k_paged_tile(ThvmPagedArgs a, P
     const uint32_t cb = 64 * d + 32 * (lane >> 4 & 1) + 8 * (lane & 3);
     va[d] = v_at<HD>(4 * h + (lane & 15) / 4, cb >> 4) + (cb & 15);
   }
-  const float qs = a.scale * LOG2E;
   float m = -INFINITY, l = 0.0f;
   f32x16_t acc[DB];
 #pragma unroll
@@ -179,7 +187,7 @@ __global__ __launch_bounds__(PP_THREADS, 2) void k_paged_tile(ThvmPagedArgs a, P
     for (int rb = 0; rb < 2; rb++)
 #pragma unroll
       for (int i = 0; i < 16; i++) {
-        float x = sc[rb][i] * qs;
+        float x = sc[rb][i];                               // (scaled in the exponent)
         if (MASK) {
           const int r = 32 * rb + 8 * (i / 4) + 4 * h + i % 4;
           if (rr + r >= lim || (holes >> (r / 16) & 1)) x = -INFINITY;
@@ -187,7 +195,7 @@ __global__ __launch_bounds__(PP_THREADS, 2) void k_paged_tile(ThvmPagedArgs a, P
         sc[rb][i] = x;
         mx = fmaxf(mx, x);
       }
-    mx = fmaxf(mx, xor32_f(mx));
+    mx = fmaxf(mx, xor32_f(mx)) * qs;
     if (__builtin_amdgcn_ballot_w64(mx > m + 6.0f)) {      // (m = -inf: any score)
       const float mn = fmaxf(m, mx), f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
       l *= f;
@@ -204,9 +212,8 @@ __global__ __launch_bounds__(PP_THREADS, 2) void k_paged_tile(ThvmPagedArgs a, P
     for (int rb = 0; rb < 2; rb++)
 #pragma unroll
       for (int i = 0; i < 16; i += 2) {
-        const float x = __builtin_amdgcn_exp2f(sc[rb][i] - mb), y = __builtin_amdgcn_exp2f(sc[rb][i + 1] - mb);
-        ls[(i / 2) & 3] += x + y;
-        pk[rb][i / 2] = P::pk(x, y);
+        pk[rb][i / 2] = P::pk(__builtin_amdgcn_exp2f(fmaf(sc[rb][i], qs, -mb)), __builtin_amdgcn_exp2f(fmaf(sc[rb][i + 1], qs, -mb)));
+        ls[(i / 2) & 3] = P::sum2(pk[rb][i / 2], ls[(i / 2) & 3]);
       }
     l += (ls[0] + ls[1]) + (ls[2] + ls[3]);
 #pragma unroll
@@ -305,7 +312,7 @@ __global__ __launch_bounds__(PP_THREADS, 2) void k_paged_tile(ThvmPagedArgs a, P
         *(uint2 *)(o + 32 * d + 8 * q) = make_uint2(P::pk(acc[d][4 * q] * inv, acc[d][4 * q + 1] * inv),
                                                     P::pk(acc[d][4 * q + 2] * inv, acc[d][4 * q + 3] * inv));
   } else {
-    float *pp = a.ws + (((uint64_t)kvh * pl.units + un) * PP_COLS + 32 * wv + n) * (HD + 4);
+    float *pp = a.ws + (((uint64_t)kvh * pl.units + u.u) * PP_COLS + 32 * wv + n) * (HD + 4);
 #pragma unroll
     for (int d = 0; d < DB; d++)
 #pragma unroll
