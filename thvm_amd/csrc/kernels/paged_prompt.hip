@@ -36,6 +36,13 @@ __device__ __forceinline__ f32x16_t mfma32(const uint4 &A, const uint4 &B, f32x1
 }
 typedef short s16x4v_t __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) s16x4v_t lds_s16x4_t;
+// 16 bytes a lane from memory into LDS, the wave's lanes in consecutive places from dst
+// on (wave-uniform); offsets past the resource write zeros
+__device__ __forceinline__ void buf_lds16(buf_t r, char *dst, uint32_t off) {
+#ifdef __HIP_DEVICE_COMPILE__                              // (the host pass does not know the builtin's size)
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void *)dst, 16, off, 0, 0, 0);
+#endif
+}
 
 template <bool V> struct pp_const { static constexpr bool value = V; };
 
@@ -51,10 +58,11 @@ template <int HD, int XT, int BITS>
 __global__ __launch_bounds__(PP_THREADS, 2) void k_paged_tile(ThvmPagedArgs a, PgPlan pl) {
   typedef PgT<XT> P;
   constexpr int KS = HD / 16, DB = HD / 32, RB = BITS == 16 ? HD * 2 : HD / 2;
-  constexpr int NL = BITS == 16 ? HD / 32 : 1;             // 16-byte (4 bits, hd 64: 8-byte) loads of K a thread
+  constexpr int NL = HD / 32;                              // passes of the block over a step's K or V
   constexpr float PSH = XT == GX_BF16 ? 0.0f : 8.0f;
   constexpr uint32_t EXP = XT == GX_BF16 ? 0x7f80u : 0x7c00u;
-  __shared__ __align__(16) char lk[2][PP_STEP * HD * 2], lv[2][PP_STEP * HD * 2];
+  // (arrays apart: reads of one then need not wait for what is on its way into another)
+  __shared__ __align__(16) char lk0[PP_STEP * HD * 2], lk1[PP_STEP * HD * 2], lv0[PP_STEP * HD * 2], lv1[PP_STEP * HD * 2];
   const uint32_t kvh = blockIdx.x % a.Hkv, un = blockIdx.x / a.Hkv, G = a.H / a.Hkv;
   PgUnit u;
   if (!pg_unit(a, pl, un, false, u)) return;
@@ -88,71 +96,66 @@ __global__ __launch_bounds__(PP_THREADS, 2) void k_paged_tile(ThvmPagedArgs a, P
                     : make_uint4(qb[ks].x ^ 0x80008000u, qb[ks].y ^ 0x80008000u, qb[ks].z ^ 0x80008000u, qb[ks].w ^ 0x80008000u);
   const buf_t tb = buf_rsrc(a.table + (uint64_t)u.s * a.maxpages, a.maxpages * 4);
   const uint32_t lgp = __builtin_ctz(a.page), pm = a.page - 1, bb = pg_block_bytes(&a);
+  // rows below `all` every column of the block sees
+  const int32_t all = p0 + (int32_t)(u.tile * PP_COLS / G) + 1;
   const int nt = r1 > r0 ? (r1 - r0 + PP_STEP - 1) / PP_STEP : 0;
-  // page ids of a step's four 16-row groups, in lanes 0..3
+  // page ids of a step's four 16-row groups, in lanes 0..3; -1: none, or past the rows
   auto ids = [&](int j) {
     const int32_t r = r0 + PP_STEP * j + 16 * (lane & 3);
-    return (int32_t)buf_ld4(tb, r < r1 ? ((uint32_t)r >> lgp) * 4 : BUF_OOB);
+    const uint32_t id = buf_ld4(tb, r < r1 ? ((uint32_t)r >> lgp) * 4 : BUF_OOB);
+    return (r < r1) & (id < a.npages) ? (int32_t)id : -1;
   };
-  auto group_ok = [&](int32_t id, int j, int g) {
-    return (uint32_t)__builtin_amdgcn_readlane(id, g) < a.npages && r0 + PP_STEP * j + 16 * g < r1;
+  // The way of a step's K or V into LDS.  16 bits: straight from memory, 16 bytes a
+  // lane into consecutive places, so the XOR of the pieces is in what a lane asks for;
+  // a group's resource begins at its first row and ends at its last (rows past it and
+  // pages that are none read as zeros), which leaves a lane's offset constant.  4 bits:
+  // through registers and the codec, 32 (hd 64: 16) values a thread.
+  const uint64_t pstride = (uint64_t)a.Hkv * bb, head = (uint64_t)kvh * bb;
+  auto group = [&](const void *pool, int32_t id, int j, int g, uint32_t at, uint32_t rb) {
+    const int32_t x = __builtin_amdgcn_readlane(id, g), have = ~(x >> 31), gr = r0 + PP_STEP * j + 16 * g;
+    return buf_rsrc((const char *)pool + head + (uint32_t)(x & have) * pstride + at + ((uint32_t)gr & pm) * rb,
+                    (uint32_t)(min(r1 - gr, 16) & have) * rb);
   };
-  // what a thread stages of a step: pieces of rows tid / PR + i * rows-per-pass
-  uint4 sk[NL], sv[NL];
-  uint32_t ssc;                                            // 4 bits: K's scale byte, V's in the next
-  auto load = [&](int32_t id, int j) {
-#pragma unroll
-    for (int i = 0; i < NL; i++) {
-      // the 16-row group of this wave's rows in pass i
-      const int g = BITS == 4 ? wv : HD == 128 ? i : 2 * i + (wv >> 1);
-      const bool ok = group_ok(id, j, g);
-      const uint64_t off = ok ? pg_block(&a, __builtin_amdgcn_readlane(id, g), kvh) : 0;
-      const buf_t kr = buf_rsrc((const char *)a.kpages + off, ok ? bb : 0u), vr = buf_rsrc((const char *)a.vpages + off, ok ? bb : 0u);
-      if constexpr (BITS == 16) {
-        constexpr int PR = HD / 8;                         // pieces a row
-        const int32_t r = r0 + PP_STEP * j + tid / PR + i * (PP_THREADS / PR);
-        const uint32_t o = r < r1 ? ((uint32_t)r & pm) * RB + (tid % PR) * 16 : BUF_OOB;
-        sk[i] = buf_ld16(kr, o);
-        sv[i] = buf_ld16(vr, o);
-      } else {
-        const int32_t r = r0 + PP_STEP * j + tid / 4;
-        const uint32_t slot = (uint32_t)r & pm, pc = tid & 3;
-        const uint32_t o = r < r1 ? slot * RB + pc * (RB / 4) : BUF_OOB;
-        const uint32_t so = r < r1 ? a.page * RB + slot * (HD / 32) + pc * HD / 128 : BUF_OOB;
-        if constexpr (HD == 128) {
-          sk[i] = buf_ld16(kr, o);
-          sv[i] = buf_ld16(vr, o);
-        } else {
-          const uint2 x = buf_ld8(kr, o), y = buf_ld8(vr, o);
-          sk[i] = make_uint4(x.x, x.y, 0, 0);
-          sv[i] = make_uint4(y.x, y.y, 0, 0);
-        }
-        ssc = (uint32_t)__builtin_amdgcn_raw_buffer_load_b8(kr, so, 0, 0) |
-              (uint32_t)__builtin_amdgcn_raw_buffer_load_b8(vr, so, 0, 0) << 8;
-      }
-    }
-  };
-  auto store = [&](int b) {
+  constexpr int PR = HD / 8;                               // 16-byte pieces of a row in LDS
+  const uint32_t r16 = (tid / PR) & 15, pc = tid % PR;
+  const uint32_t ko = r16 * RB + (k_at<HD>(r16, pc) - r16 * (HD * 2)), vo = r16 * RB + (v_at<HD>(r16, pc) - r16 * (HD * 2));
+  uint4 sr;
+  uint32_t ssc;
+  auto load = [&](const void *pool, int32_t id, int j, char *dst, uint32_t off) {
     if constexpr (BITS == 16) {
-      constexpr int PR = HD / 8;
 #pragma unroll
-      for (int i = 0; i < NL; i++) {
-        const uint32_t r = tid / PR + i * (PP_THREADS / PR), c = tid % PR;
-        *(uint4 *)&lk[b][k_at<HD>(r, c)] = sk[i];
-        *(uint4 *)&lv[b][v_at<HD>(r, c)] = sv[i];
-      }
+      for (int i = 0; i < NL; i++)                         // the 16-row group of this wave's rows in pass i
+        buf_lds16(group(pool, id, j, HD == 128 ? i : 2 * i + (wv >> 1), 0, RB), &dst[(i * PP_THREADS + wv * 64) * 16], off);
     } else {
-      const uint32_t r = tid / 4, pc = tid & 3;
-      const float fk = e8m0_f(ssc & 0xffu), fv = e8m0_f(ssc >> 8);
-      const uint32_t wk[4] = {sk[0].x, sk[0].y, sk[0].z, sk[0].w}, wvv[4] = {sv[0].x, sv[0].y, sv[0].z, sv[0].w};
-#pragma unroll
-      for (int c = 0; c < HD / 32; c++) {                  // 8 values a dword of codes
-        *(uint4 *)&lk[b][k_at<HD>(r, pc * (HD / 32) + c)] =
-            make_uint4(fp4x2<XT, 0>(wk[c], fk), fp4x2<XT, 1>(wk[c], fk), fp4x2<XT, 2>(wk[c], fk), fp4x2<XT, 3>(wk[c], fk));
-        *(uint4 *)&lv[b][v_at<HD>(r, pc * (HD / 32) + c)] =
-            make_uint4(fp4x2<XT, 0>(wvv[c], fv), fp4x2<XT, 1>(wvv[c], fv), fp4x2<XT, 2>(wvv[c], fv), fp4x2<XT, 3>(wvv[c], fv));
+      const uint32_t r = (tid >> 2) & 15, p4 = tid & 3;
+      const buf_t rs = group(pool, id, j, wv, 0, RB);
+      if constexpr (HD == 128) {
+        sr = buf_ld16(rs, r * RB + p4 * (RB / 4));
+      } else {
+        const uint2 x = buf_ld8(rs, r * RB + p4 * (RB / 4));
+        sr = make_uint4(x.x, x.y, 0, 0);
       }
+      ssc = (uint32_t)__builtin_amdgcn_raw_buffer_load_b8(group(pool, id, j, wv, a.page * RB, HD / 32), r * (HD / 32) + p4 * HD / 128, 0, 0);
     }
+  };
+  auto store = [&](char *dst, auto at) {
+    if constexpr (BITS == 4) {
+      const uint32_t r = tid / 4, p4 = tid & 3, w[4] = {sr.x, sr.y, sr.z, sr.w};
+      const float f = e8m0_f(ssc);
+#pragma unroll
+      for (int c = 0; c < HD / 32; c++)                    // 8 values a dword of codes
+        *(uint4 *)&dst[at(r, p4 * (HD / 32) + c)] =
+            make_uint4(fp4x2<XT, 0>(w[c], f), fp4x2<XT, 1>(w[c], f), fp4x2<XT, 2>(w[c], f), fp4x2<XT, 3>(w[c], f));
+    }
+  };
+  auto load_k = [&](int32_t id, int j, char *dst) { load(a.kpages, id, j, dst, ko); };
+  auto load_v = [&](int32_t id, int j, char *dst) { load(a.vpages, id, j, dst, vo); };
+  auto store_k = [&](char *dst) { store(dst, [](uint32_t r, uint32_t c) { return k_at<HD>(r, c); }); };
+  auto store_v = [&](char *dst) { store(dst, [](uint32_t r, uint32_t c) { return v_at<HD>(r, c); }); };
+  // the block's own LDS loads done, then the other waves'
+  auto arrive = [] {
+    __builtin_amdgcn_s_waitcnt(0x0f70);                    // vmcnt(0)
+    __syncthreads();
   };
   // operand addresses: a piece's XOR depends on the lane alone, rows add constants
   uint32_t ka[KS], va[DB];
@@ -170,31 +173,43 @@ __global__ __launch_bounds__(PP_THREADS, 2) void k_paged_tile(ThvmPagedArgs a, P
   for (int d = 0; d < DB; d++)
 #pragma unroll
     for (int i = 0; i < 16; i++) acc[d][i] = 0.0f;
-  auto step = [&](auto masked, int b, int j, uint32_t holes) {
-    constexpr bool MASK = decltype(masked)::value;
-    f32x16_t sc[2];
-#pragma unroll
-    for (int rb = 0; rb < 2; rb++) {
-#pragma unroll
-      for (int i = 0; i < 16; i++) sc[rb][i] = 0.0f;
-#pragma unroll
-      for (int ks = 0; ks < KS; ks++)
-        sc[rb] = mfma32<XT>(*(const uint4 *)&lk[b][ka[ks] + 32 * rb * (HD * 2)], qb[ks], sc[rb]);
-    }
-    const int32_t rr = r0 + PP_STEP * j;
-    float mx = -INFINITY;
+  struct Sc { f32x16_t v[2]; };
+  auto scores = [&](const char *lk, Sc &S) {
 #pragma unroll
     for (int rb = 0; rb < 2; rb++)
 #pragma unroll
-      for (int i = 0; i < 16; i++) {
-        float x = sc[rb][i];                               // (scaled in the exponent)
-        if (MASK) {
-          const int r = 32 * rb + 8 * (i / 4) + 4 * h + i % 4;
-          if (rr + r >= lim || (holes >> (r / 16) & 1)) x = -INFINITY;
+      for (int i = 0; i < 16; i++) S.v[rb][i] = 0.0f;
+#pragma unroll
+    for (int ks = 0; ks < KS; ks++) {
+#pragma unroll
+      for (int rb = 0; rb < 2; rb++)
+        S.v[rb] = mfma32<XT>(*(const uint4 *)&lk[ka[ks] + 32 * rb * (HD * 2)], qb[ks], S.v[rb]);
+    }
+  };
+  // the scores that a column does not see to -inf, and the largest
+  auto top = [&](auto masked, int j, uint32_t holes, Sc &S) {
+    constexpr bool MASK = decltype(masked)::value;
+    float mx = -INFINITY;
+    if (MASK) {
+      const int32_t left = lim - (r0 + PP_STEP * j) - 4 * h;
+      int32_t lg[4];
+#pragma unroll
+      for (int g = 0; g < 4; g++) lg[g] = holes >> g & 1 ? 0 : left;
+#pragma unroll
+      for (int rb = 0; rb < 2; rb++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+          const int r = 32 * rb + 8 * (i / 4) + i % 4;     // (4 h is in left)
+          S.v[rb][i] = r < lg[r / 16] ? S.v[rb][i] : -INFINITY;
         }
-        sc[rb][i] = x;
-        mx = fmaxf(mx, x);
-      }
+    }
+#pragma unroll
+    for (int rb = 0; rb < 2; rb++)
+#pragma unroll
+      for (int i = 0; i < 16; i++) mx = fmaxf(mx, S.v[rb][i]);
+    return mx;
+  };
+  auto move = [&](float mx) {
     mx = fmaxf(mx, xor32_f(mx)) * qs;
     if (__builtin_amdgcn_ballot_w64(mx > m + 6.0f)) {      // (m = -inf: any score)
       const float mn = fmaxf(m, mx), f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
@@ -205,100 +220,154 @@ __global__ __launch_bounds__(PP_THREADS, 2) void k_paged_tile(ThvmPagedArgs a, P
         for (int i = 0; i < 16; i++) acc[d][i] *= f;
       m = mn;
     }
+  };
+  auto expo = [&](const Sc &S, uint32_t pk[2][8]) {
     const float mb = (m == -INFINITY ? 0.0f : m) - PSH;
-    float ls[4] = {0.f, 0.f, 0.f, 0.f};
-    uint32_t pk[2][8];
+    float ls[2] = {0.f, 0.f};
 #pragma unroll
     for (int rb = 0; rb < 2; rb++)
 #pragma unroll
       for (int i = 0; i < 16; i += 2) {
-        pk[rb][i / 2] = P::pk(__builtin_amdgcn_exp2f(fmaf(sc[rb][i], qs, -mb)), __builtin_amdgcn_exp2f(fmaf(sc[rb][i + 1], qs, -mb)));
-        ls[(i / 2) & 3] = P::sum2(pk[rb][i / 2], ls[(i / 2) & 3]);
+        pk[rb][i / 2] = P::pk(__builtin_amdgcn_exp2f(fmaf(S.v[rb][i], qs, -mb)), __builtin_amdgcn_exp2f(fmaf(S.v[rb][i + 1], qs, -mb)));
+        ls[i / 2 & 1] = P::sum2(pk[rb][i / 2], ls[i / 2 & 1]);
       }
-    l += (ls[0] + ls[1]) + (ls[2] + ls[3]);
+    l += ls[0] + ls[1];
+  };
+  auto mix = [&](auto masked, const char *lv, const uint32_t pk[2][8]) {
+    constexpr bool MASK = decltype(masked)::value;
 #pragma unroll
     for (int s = 0; s < 4; s++) {                          // 16 rows each
       const uint4 B = make_uint4(pk[s / 2][4 * (s & 1)], pk[s / 2][4 * (s & 1) + 1], pk[s / 2][4 * (s & 1) + 2],
                                  pk[s / 2][4 * (s & 1) + 3]);
 #pragma unroll
       for (int d = 0; d < DB; d++) {
-        uint4 A;
-        {
-          // rows 16 s + 4 h .. + 3 and those 8 further on, in the order of P's
-          typedef uint32_t u2_t __attribute__((ext_vector_type(2)));
-          const u2_t x = __builtin_bit_cast(u2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                                                      (lds_s16x4_t *)&lv[b][va[d] + 16 * s * (HD * 2)]));
-          const u2_t y = __builtin_bit_cast(u2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                                                      (lds_s16x4_t *)&lv[b][va[d] + (16 * s + 8) * (HD * 2)]));
-          A = make_uint4(x[0], x[1], y[0], y[1]);
-        }
+        // rows 16 s + 4 h .. + 3 and those 8 further on, in the order of P's
+        typedef uint32_t u2_t __attribute__((ext_vector_type(2)));
+        const u2_t x = __builtin_bit_cast(u2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                                    (lds_s16x4_t *)&lv[va[d] + 16 * s * (HD * 2)]));
+        const u2_t y = __builtin_bit_cast(u2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                                    (lds_s16x4_t *)&lv[va[d] + (16 * s + 8) * (HD * 2)]));
+        uint4 A = make_uint4(x[0], x[1], y[0], y[1]);
+        uint32_t big = 0;                                  // the largest exponents of its halves
         if (MASK) {
-          // A zero p times a V that is not finite is NaN: where a step has masked
-          // rows, such values leave the product and come back as +inf, -inf or (both)
-          // NaN in the columns where one has a p above zero.
-          uint32_t w[4] = {A.x, A.y, A.z, A.w}, odd = 0;
-#pragma unroll
-          for (int i = 0; i < 4; i++) odd |= (w[i] & EXP) == EXP || (w[i] >> 16 & EXP) == EXP;
-          if (__builtin_amdgcn_ballot_w64(odd)) {          // wave-uniform
+          typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+          const uint32_t ee = EXP | EXP << 16;
+          big = __builtin_bit_cast(uint32_t, __builtin_elementwise_max(
+              __builtin_elementwise_max(__builtin_bit_cast(u16x2, A.x & ee), __builtin_bit_cast(u16x2, A.y & ee)),
+              __builtin_elementwise_max(__builtin_bit_cast(u16x2, A.z & ee), __builtin_bit_cast(u16x2, A.w & ee))));
+        }
+        if (MASK && __builtin_amdgcn_ballot_w64((big & 0xffffu) == EXP || big >> 16 == EXP)) {   // wave-uniform
+          // A zero p times a V that is not finite is NaN: such values leave the product
+          // and come back as +inf, -inf or (both) NaN in the columns where one has a p
+          // above zero.
+          uint32_t w[4] = {A.x, A.y, A.z, A.w};
 #pragma unroll 1
-            for (int sign = 0; sign < 2; sign++) {
-              const uint32_t one = XT == GX_BF16 ? 0x3f80u : 0x3c00u, other = sign ? EXP : EXP | 0x8000u;
-              uint32_t t[4];
-#pragma unroll
-              for (int i = 0; i < 4; i++) {
-                const uint32_t x = w[i] & 0xffffu, y = w[i] >> 16;
-                t[i] = ((x & EXP) == EXP && x != other ? one : 0u) | ((y & EXP) == EXP && y != other ? one << 16 : 0u);
-              }
-              f32x16_t z;
-#pragma unroll
-              for (int i = 0; i < 16; i++) z[i] = 0.0f;
-              z = mfma32<XT>(make_uint4(t[0], t[1], t[2], t[3]), B, z);
-#pragma unroll
-              for (int i = 0; i < 16; i++) acc[d][i] += z[i] > 0.0f ? (sign ? -INFINITY : INFINITY) : 0.0f;
-            }
+          for (int sign = 0; sign < 2; sign++) {
+            const uint32_t one = XT == GX_BF16 ? 0x3f80u : 0x3c00u, other = sign ? EXP : EXP | 0x8000u;
+            uint32_t t[4];
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-              if ((w[i] & EXP) == EXP) w[i] &= 0xffff0000u;
-              if ((w[i] >> 16 & EXP) == EXP) w[i] &= 0xffffu;
+              const uint32_t e = w[i] & 0xffffu, o = w[i] >> 16;
+              t[i] = ((e & EXP) == EXP && e != other ? one : 0u) | ((o & EXP) == EXP && o != other ? one << 16 : 0u);
             }
-            A = make_uint4(w[0], w[1], w[2], w[3]);
+            f32x16_t z;
+#pragma unroll
+            for (int i = 0; i < 16; i++) z[i] = 0.0f;
+            z = mfma32<XT>(make_uint4(t[0], t[1], t[2], t[3]), B, z);
+#pragma unroll
+            for (int i = 0; i < 16; i++) acc[d][i] += z[i] > 0.0f ? (sign ? -INFINITY : INFINITY) : 0.0f;
           }
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            if ((w[i] & EXP) == EXP) w[i] &= 0xffff0000u;
+            if ((w[i] >> 16 & EXP) == EXP) w[i] &= 0xffffu;
+          }
+          A = make_uint4(w[0], w[1], w[2], w[3]);
         }
         acc[d] = mfma32<XT>(A, B, acc[d]);
       }
     }
   };
-  int32_t id = ids(0), idn = ids(1);
+  // Steps overlap: while a step's scores go through the exponent the next one's are
+  // multiplied (K runs a step ahead of V), and while its values are multiplied the
+  // next one's scores are searched for their maximum.  First the steps that every
+  // column of the block sees whole, two at a time, then (from the first page that is
+  // none, or the first position of the tile) the others.
+  int32_t i0 = ids(0), i1 = ids(1), i2 = ids(2);           // page ids of steps j, j + 1, j + 2
+  Sc S0, S1;
   if (nt) {
-    load(id, 0);
-    store(0);
+    load_k(i0, 0, lk0);
+    store_k(lk0);
+    load_v(i0, 0, lv0);
+    store_v(lv0);
+    load_k(i1, 1, lk1);
+    store_k(lk1);
   }
-  __syncthreads();
-  // steps that every column of the block sees whole, then (from the first page that
-  // is none, or the first position of the tile) the others
-  const int32_t all = p0 + (int32_t)(u.tile * PP_COLS / G) + 1;
+  arrive();
   int j = 0;
-  auto holes_of = [&](int32_t i) {
+  auto holes_of = [&](int32_t id) {
     uint32_t o = 0;
 #pragma unroll
-    for (int g = 0; g < 4; g++) o |= group_ok(i, j, g) ? 0u : 1u << g;
+    for (int g = 0; g < 4; g++) o |= (uint32_t)__builtin_amdgcn_readlane(id, g) >> 31 << g;
     return o;
   };
-  auto next = [&](auto run) {                              // the next step's bytes on their way meanwhile
-    id = idn;
-    idn = ids(j + 2);
-    const bool more = j + 1 < nt;
-    if (more) load(id, j + 1);
-    run();
-    if (more) store((j + 1) & 1);
-    __syncthreads();
+  auto full = [&](int32_t id, int j) { return r0 + PP_STEP * (j + 1) <= min(all, r1) && holes_of(id) == 0; };
+  auto step = [&](auto masked, Sc &S, Sc &N, char *k0, char *k1, char *v0, char *v1) {
+    constexpr bool MASK = decltype(masked)::value;
+    const int32_t rr = r0 + PP_STEP * j;
+    const bool seen = !MASK || rr < whi, seen1 = !MASK || rr + PP_STEP < whi;   // wave-uniform
+    uint32_t pk[2][8];
+    load_k(i2, j + 2, k0);
+    const int32_t i3 = ids(j + 3);
+    __builtin_amdgcn_sched_barrier(0);
+    if (seen1) scores(k1, N);
+    if (seen) expo(S, pk);
+    if (!MASK) {                                           // pieces of K three ahead of their products, exponents between
+      __builtin_amdgcn_sched_group_barrier(0x100, 3, 0);
+#pragma unroll
+      for (int q = 0; q < 2 * KS; q++) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x002, 32 / KS, 0);
+        __builtin_amdgcn_sched_group_barrier(0x400, 16 / KS, 0);
+      }
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    store_k(k0);
+    load_v(i1, j + 1, v1);
+    __builtin_amdgcn_sched_barrier(0);
+    float mx = -INFINITY;
+    if (seen) mix(masked, v0, pk);
+    if (seen1) mx = top(masked, j + 1, MASK ? holes_of(i1) : 0, N);
+    if (!MASK) {
+      __builtin_amdgcn_sched_group_barrier(0x100, 6, 0);
+#pragma unroll
+      for (int q = 0; q < 4 * DB; q++) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+        __builtin_amdgcn_sched_group_barrier(0x002, 2, 0);
+      }
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    store_v(v1);
+    if (seen1) move(mx);
+    arrive();
+    i0 = i1;
+    i1 = i2;
+    i2 = i3;
     j++;
   };
-  while (j < nt && r0 + PP_STEP * (j + 1) <= min(all, r1) && holes_of(id) == 0)
-    next([&] { step(pp_const<false>{}, j & 1, j, 0); });
+  if (nt) {
+    scores(lk0, S0);
+    move(top(pp_const<true>{}, 0, holes_of(i0), S0));
+  }
+  while (j + 2 < nt && full(i0, j) && full(i1, j + 1) && full(i2, j + 2)) {
+    step(pp_const<false>{}, S0, S1, lk0, lk1, lv0, lv1);
+    step(pp_const<false>{}, S1, S0, lk1, lk0, lv1, lv0);
+  }
   while (j < nt) {
-    const uint32_t holes = holes_of(id);
-    next([&] { if (r0 + PP_STEP * j < whi) step(pp_const<true>{}, j & 1, j, holes); });   // wave-uniform
+    step(pp_const<true>{}, S0, S1, lk0, lk1, lv0, lv1);
+    if (j < nt) step(pp_const<true>{}, S1, S0, lk1, lk0, lv1, lv0);
   }
   if (!live) return;
   l += xor32_f(l);
