@@ -103,26 +103,32 @@ __global__ __launch_bounds__(PP_THREADS, 2) void k_paged_tile(ThvmPagedArgs a, P
   auto ids = [&](int j) {
     const int32_t r = r0 + PP_STEP * j + 16 * (lane & 3);
     const uint32_t id = buf_ld4(tb, r < r1 ? ((uint32_t)r >> lgp) * 4 : BUF_OOB);
-    return (r < r1) & (id < a.npages) ? (int32_t)id : -1;
+    return ((r < r1) & (id < a.npages)) ? (int32_t)id : -1;
   };
   // The way of a step's K or V into LDS.  16 bits: straight from memory, 16 bytes a
   // lane into consecutive places, so the XOR of the pieces is in what a lane asks for;
   // a group's resource begins at its first row and ends at its last (rows past it and
   // pages that are none read as zeros), which leaves a lane's offset constant.  4 bits:
   // through registers and the codec, 32 (hd 64: 16) values a thread.
-  const uint64_t pstride = (uint64_t)a.Hkv * bb, head = (uint64_t)kvh * bb;
-  auto group = [&](const void *pool, int32_t id, int j, int g, uint32_t at, uint32_t rb) {
+  const uint64_t pstride = a.Hkv * bb, head = (uint64_t)kvh * bb;
+  const uint32_t ps32 = (uint32_t)pstride;
+  auto group = [&](const void *pool, int32_t id, int j, int g, uint32_t at, uint32_t rb, int32_t most = 16) {
     const int32_t x = __builtin_amdgcn_readlane(id, g), have = ~(x >> 31), gr = r0 + PP_STEP * j + 16 * g;
-    return buf_rsrc((const char *)pool + head + (uint32_t)(x & have) * pstride + at + ((uint32_t)gr & pm) * rb,
-                    (uint32_t)(min(r1 - gr, 16) & have) * rb);
+    return buf_rsrc((const char *)pool + head + (uint64_t)(uint32_t)(x & have) * ps32 + at + ((uint32_t)gr & pm) * rb,
+                    (uint32_t)(min(r1 - gr, most) & have) * rb);
   };
   constexpr int PR = HD / 8;                               // 16-byte pieces of a row in LDS
   const uint32_t r16 = (tid / PR) & 15, pc = tid % PR;
   const uint32_t ko = r16 * RB + (k_at<HD>(r16, pc) - r16 * (HD * 2)), vo = r16 * RB + (v_at<HD>(r16, pc) - r16 * (HD * 2));
-  uint4 sr;
-  uint32_t ssc;
-  auto load = [&](const void *pool, int32_t id, int j, char *dst, uint32_t off) {
+  struct Reg { uint4 c; uint32_t s; } rk, rv;
+  auto load = [&](const void *pool, int32_t id, int j, char *dst, uint32_t off, Reg &x) {
     if constexpr (BITS == 16) {
+      if (a.page >= PP_STEP) {                             // the whole step in one page
+        const buf_t rs = group(pool, id, j, 0, 0, RB, PP_STEP);
+#pragma unroll
+        for (int i = 0; i < NL; i++)
+          buf_lds16(rs, &dst[(i * PP_THREADS + wv * 64) * 16], off + (wv * 64 / PR / 16 * 16 + i * (PP_THREADS / PR)) * RB);
+      } else
 #pragma unroll
       for (int i = 0; i < NL; i++)                         // the 16-row group of this wave's rows in pass i
         buf_lds16(group(pool, id, j, HD == 128 ? i : 2 * i + (wv >> 1), 0, RB), &dst[(i * PP_THREADS + wv * 64) * 16], off);
@@ -130,28 +136,28 @@ __global__ __launch_bounds__(PP_THREADS, 2) void k_paged_tile(ThvmPagedArgs a, P
       const uint32_t r = (tid >> 2) & 15, p4 = tid & 3;
       const buf_t rs = group(pool, id, j, wv, 0, RB);
       if constexpr (HD == 128) {
-        sr = buf_ld16(rs, r * RB + p4 * (RB / 4));
+        x.c = buf_ld16(rs, r * RB + p4 * (RB / 4));
       } else {
-        const uint2 x = buf_ld8(rs, r * RB + p4 * (RB / 4));
-        sr = make_uint4(x.x, x.y, 0, 0);
+        const uint2 y = buf_ld8(rs, r * RB + p4 * (RB / 4));
+        x.c = make_uint4(y.x, y.y, 0, 0);
       }
-      ssc = (uint32_t)__builtin_amdgcn_raw_buffer_load_b8(group(pool, id, j, wv, a.page * RB, HD / 32), r * (HD / 32) + p4 * HD / 128, 0, 0);
+      x.s = (uint32_t)__builtin_amdgcn_raw_buffer_load_b8(group(pool, id, j, wv, a.page * RB, HD / 32), r * (HD / 32) + p4 * HD / 128, 0, 0);
     }
   };
-  auto store = [&](char *dst, auto at) {
+  auto store = [&](char *dst, auto at, const Reg &x) {
     if constexpr (BITS == 4) {
-      const uint32_t r = tid / 4, p4 = tid & 3, w[4] = {sr.x, sr.y, sr.z, sr.w};
-      const float f = e8m0_f(ssc);
+      const uint32_t r = tid / 4, p4 = tid & 3, w[4] = {x.c.x, x.c.y, x.c.z, x.c.w};
+      const float f = e8m0_f(x.s);
 #pragma unroll
       for (int c = 0; c < HD / 32; c++)                    // 8 values a dword of codes
         *(uint4 *)&dst[at(r, p4 * (HD / 32) + c)] =
             make_uint4(fp4x2<XT, 0>(w[c], f), fp4x2<XT, 1>(w[c], f), fp4x2<XT, 2>(w[c], f), fp4x2<XT, 3>(w[c], f));
     }
   };
-  auto load_k = [&](int32_t id, int j, char *dst) { load(a.kpages, id, j, dst, ko); };
-  auto load_v = [&](int32_t id, int j, char *dst) { load(a.vpages, id, j, dst, vo); };
-  auto store_k = [&](char *dst) { store(dst, [](uint32_t r, uint32_t c) { return k_at<HD>(r, c); }); };
-  auto store_v = [&](char *dst) { store(dst, [](uint32_t r, uint32_t c) { return v_at<HD>(r, c); }); };
+  auto load_k = [&](int32_t id, int j, char *dst) { load(a.kpages, id, j, dst, ko, rk); };
+  auto load_v = [&](int32_t id, int j, char *dst) { load(a.vpages, id, j, dst, vo, rv); };
+  auto store_k = [&](char *dst) { store(dst, [](uint32_t r, uint32_t c) { return k_at<HD>(r, c); }, rk); };
+  auto store_v = [&](char *dst) { store(dst, [](uint32_t r, uint32_t c) { return v_at<HD>(r, c); }, rv); };
   // the block's own LDS loads done, then the other waves'
   auto arrive = [] {
     __builtin_amdgcn_s_waitcnt(0x0f70);                    // vmcnt(0)
@@ -318,6 +324,7 @@ __global__ __launch_bounds__(PP_THREADS, 2) void k_paged_tile(ThvmPagedArgs a, P
     const bool seen = !MASK || rr < whi, seen1 = !MASK || rr + PP_STEP < whi;   // wave-uniform
     uint32_t pk[2][8];
     load_k(i2, j + 2, k0);
+    load_v(i1, j + 1, v1);
     const int32_t i3 = ids(j + 3);
     __builtin_amdgcn_sched_barrier(0);
     if (seen1) scores(k1, N);
@@ -334,7 +341,6 @@ __global__ __launch_bounds__(PP_THREADS, 2) void k_paged_tile(ThvmPagedArgs a, P
     }
     __builtin_amdgcn_sched_barrier(0);
     store_k(k0);
-    load_v(i1, j + 1, v1);
     __builtin_amdgcn_sched_barrier(0);
     float mx = -INFINITY;
     if (seen) mix(masked, v0, pk);
