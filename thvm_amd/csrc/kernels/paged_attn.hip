@@ -8,8 +8,91 @@
 // into chunks whose partial sums k_paged_merge adds.  Softmax statistics and sums
 // are f32.
 #include "paged_core.h"
+#include "coh.h"
 
 #define LOG2E 1.4426950408889634f
+
+// Columns of a tile from their chunks' partials (sum, m, l), in a fixed order.  HD /
+// 4 lanes take a chunk; NP such groups of a block take every NP-th chunk of one
+// column and meet in LDS, its other groups have other columns, from c0 on and (all
+// of the tile's CT, COH) in rounds.  COH: partials of blocks of this launch, read past
+// the caches.
+template <int HD, int XT, int CT, int NP, bool COH>
+__device__ __forceinline__ void pa_fold(const ThvmPagedArgs &a, const PgPlan &pl, const PgUnit &u, uint32_t kvh,
+                                        float4 (*ls)[HD / 4], float *lm, float *ll, uint32_t c0 = 0) {
+  typedef PgT<XT> P;
+  constexpr int LN = HD / 4, NG = 256 / LN, CB = NG / NP, BT = 8;   // lanes a chunk, groups, columns at once, loads ahead
+  const uint32_t g = threadIdx.x / LN, x = threadIdx.x % LN, part = g % NP, G = a.H / a.Hkv;
+  const uint64_t st = (uint64_t)CT * (HD + 4);
+  const float *const base = a.ws + ((uint64_t)kvh * pl.units + u.first) * st;
+  for (uint32_t c = c0 + g / NP; c < (COH ? (uint32_t)CT : c0 + CB); c += CB) {   // (as many rounds for every thread)
+    const uint32_t cc = u.tile * pl.ct + c;
+    const bool live = (int32_t)(cc / G) < u.q.r1 - u.q.r0;
+    const float *pp = base + (uint64_t)c * (HD + 4);
+    float m = -INFINITY, l = 0.0f;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (uint32_t k0 = part; live && k0 < u.nchunk; k0 += NP * BT) {
+      float4 w[BT];
+      float2 ml[BT];
+#pragma unroll
+      for (int t = 0; t < BT; t++) {
+        const uint32_t k = min(k0 + t * NP, u.nchunk - 1); // (past the last: read again, not added)
+        if (COH) {                                         // (a wave-uniform base: the launcher keeps offsets below 2 GiB)
+          const uint32_t o = (k * CT + c) * (HD + 4) * 4;
+          const uint4 q = coh_ld16(base, o + x * 16);
+          const uint2 e = coh_ld8(base, o + HD * 4);
+          w[t] = make_float4(__uint_as_float(q.x), __uint_as_float(q.y), __uint_as_float(q.z), __uint_as_float(q.w));
+          ml[t] = make_float2(__uint_as_float(e.x), __uint_as_float(e.y));
+        } else {
+          w[t] = *(const float4 *)(pp + k * st + 4 * x);
+          ml[t] = *(const float2 *)(pp + k * st + HD);
+        }
+      }
+#pragma unroll
+      for (int t = 0; t < BT; t++) {
+        if (k0 + t * NP >= u.nchunk) break;
+        const float mn = fmaxf(m, ml[t].x), f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn),
+                    e = ml[t].x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml[t].x - mn);
+        v.x = v.x * f + w[t].x * e;
+        v.y = v.y * f + w[t].y * e;
+        v.z = v.z * f + w[t].z * e;
+        v.w = v.w * f + w[t].w * e;
+        l = l * f + ml[t].y * e;
+        m = mn;
+      }
+    }
+    if (NP > 1) {
+      ls[g][x] = v;
+      if (x == 0) { lm[g] = m; ll[g] = l; }
+      __syncthreads();
+      if (part == 0) {
+        float M = -INFINITY;
+#pragma unroll
+        for (int k = 0; k < NP; k++) M = fmaxf(M, lm[g + k]);
+        l = 0.0f;
+        v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int k = 0; k < NP; k++) {
+          const float f = lm[g + k] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(lm[g + k] - M);
+          v.x += ls[g + k][x].x * f;
+          v.y += ls[g + k][x].y * f;
+          v.z += ls[g + k][x].z * f;
+          v.w += ls[g + k][x].w * f;
+          l += ll[g + k] * f;
+        }
+      }
+      __syncthreads();
+    }
+    if (!live || part) continue;
+    const float inv = l != 0.0f ? 1.0f / l : 0.0f;
+    *(uint2 *)((uint16_t *)a.out + ((uint64_t)(u.q.r0 + cc / G) * a.H + kvh * G + cc % G) * HD + 4 * x) =
+        make_uint2(P::pk(v.x * inv, v.y * inv), P::pk(v.z * inv, v.w * inv));
+  }
+}
+
+// arrivals at a tile's hand-off: zero before the first launch, left zero by each
+#define PA_COUNTERS ((1u << 20) + 2048)
+static __device__ uint32_t pa_arrived[PA_COUNTERS];
 
 // ---- a few columns: the split -------------------------------------------------
 // k_paged_split: a unit is one tile of at most 16 columns (rows x query heads of
@@ -66,62 +149,69 @@ __global__ __launch_bounds__(PS_THREADS, 2) void k_paged_split(ThvmPagedArgs a, 
   }
   const buf_t tb = buf_rsrc(a.table + (uint64_t)u.s * a.maxpages, a.maxpages * 4);
   const uint32_t lgp = __builtin_ctz(a.page), pm = a.page - 1, bb = pg_block_bytes(&a);
+  const uint64_t head = (uint64_t)kvh * bb;
+  const uint32_t pstride = a.Hkv * bb;                     // (below 2^28)
   auto row_of = [&](int it, int t) { return r0 + 256 * it + 64 * t + 16 * wv; };
-  // page ids of the four tiles, in lanes 0..3
+  // page ids of a step's four tiles, in lanes 0..3; -1: none, or past the chunk's rows
   auto ids = [&](int it) {
     const int32_t r = row_of(it, lane & 3);
-    return (int32_t)buf_ld4(tb, r < r1 ? ((uint32_t)r >> lgp) * 4 : BUF_OOB);
+    const uint32_t id = buf_ld4(tb, r < r1 ? ((uint32_t)r >> lgp) * 4 : BUF_OOB);
+    return ((r < r1) & (id < a.npages)) ? (int32_t)id : -1;
   };
   PsRegs<HD, BITS> R;
-  uint64_t off[4];                                         // a tile's block in the pools, and its bytes (0: no page)
-  uint32_t rng[4];
+  // A tile's place in the pools: its page and first slot, and how many rows it has (0:
+  // no page).  16 bits: its resources begin at its first row and end at its last, so
+  // what lies past them reads as zeros.  4 bits: they are the page's block (or empty);
+  // rows past the last have a p of zero, and their scales are taken as zero below.
+  struct Tile { uint64_t page; uint32_t slot, rows; } T[4];
   auto place = [&](int32_t id, int it) {
 #pragma unroll
     for (int t = 0; t < 4; t++) {
-      const uint32_t i = (uint32_t)__builtin_amdgcn_readlane(id, t);
-      const bool ok = i < a.npages && row_of(it, t) < r1;
-      rng[t] = ok ? bb : 0u;
-      off[t] = ok ? pg_block(&a, (int32_t)i, kvh) : 0;
+      const int32_t x = __builtin_amdgcn_readlane(id, t), have = ~(x >> 31), r = row_of(it, t);
+      T[t].page = (uint64_t)(uint32_t)(x & have) * pstride + head;
+      T[t].slot = (uint32_t)r & pm;
+      T[t].rows = (uint32_t)(min(r1 - r, 16) & have);
     }
   };
-  auto issue_k = [&](int it) {
+  auto res = [&](const void *pool, int t) {
+    if (BITS == 16) return buf_rsrc((const char *)pool + T[t].page + T[t].slot * RB, T[t].rows * RB);
+    return buf_rsrc((const char *)pool + T[t].page, T[t].rows ? bb : 0u);
+  };
+  const uint32_t ko = lc * RB + (BITS == 16 ? 16 : RB / 4) * lg, vo = 4 * lg * RB + RB / 16 * lc;
+  const uint32_t kso = lc * (HD / 32) + lg * HD / 128, vso = 4 * lg * (HD / 32), sbase = a.page * RB;
+  auto issue_k = [&]() {
 #pragma unroll
     for (int t = 0; t < 4; t++) {
-      const buf_t rs = buf_rsrc((const char *)a.kpages + off[t], rng[t]);
-      const int32_t r = row_of(it, t) + lc;
-      const uint32_t slot = ((uint32_t)row_of(it, t) & pm) + lc;
+      const buf_t rs = res(a.kpages, t);
       if constexpr (BITS == 16) {
 #pragma unroll
-        for (int ks = 0; ks < KS; ks++)
-          R.k[t][ks] = buf_ld_stream16(rs, r < r1 ? slot * RB + 16 * lg + 64 * ks : BUF_OOB);
+        for (int ks = 0; ks < KS; ks++) R.k[t][ks] = buf_ld_stream16(rs, ko + 64 * ks);
       } else {
-        if constexpr (HD == 128) R.k[t] = buf_ld_stream16(rs, r < r1 ? slot * RB + 16 * lg : BUF_OOB);
-        else R.k[t] = buf_ld8(rs, r < r1 ? slot * RB + 8 * lg : BUF_OOB);
-        R.ks[t] = __builtin_amdgcn_raw_buffer_load_b8(rs, r < r1 ? a.page * RB + slot * (HD / 32) + lg * HD / 128 : BUF_OOB, 0, 0);
+        const uint32_t so = T[t].slot * RB, ss = sbase + T[t].slot * (HD / 32);
+        if constexpr (HD == 128) R.k[t] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(rs, ko, so, 2));
+        else R.k[t] = __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(rs, ko, so, 0));
+        R.ks[t] = __builtin_amdgcn_raw_buffer_load_b8(rs, kso, ss, 0);
       }
     }
   };
-  auto issue_v = [&](int it) {
+  auto issue_v = [&]() {
 #pragma unroll
     for (int t = 0; t < 4; t++) {
-      const buf_t rs = buf_rsrc((const char *)a.vpages + off[t], rng[t]);
-      const int32_t r = row_of(it, t) + 4 * lg;
-      const uint32_t slot = ((uint32_t)row_of(it, t) & pm) + 4 * lg;
+      const buf_t rs = res(a.vpages, t);
+      const uint32_t so = T[t].slot * RB, ss = sbase + T[t].slot * (HD / 32);
 #pragma unroll
       for (int j = 0; j < 4; j++) {
         if constexpr (BITS == 16) {
-          const uint32_t o = r + j < r1 ? (slot + j) * RB + EC * 2 * lc : BUF_OOB;
-          if constexpr (HD == 128) R.v[t][j] = buf_ld_stream16(rs, o);
-          else R.v[t][j] = buf_ld8(rs, o);
+          if constexpr (HD == 128) R.v[t][j] = buf_ld_stream16(rs, vo + j * RB);
+          else R.v[t][j] = buf_ld8(rs, vo + j * RB);
         } else {
-          const uint32_t o = r + j < r1 ? (slot + j) * RB + EC / 2 * lc : BUF_OOB;
-          R.v[t][j] = HD == 128 ? buf_ld4(rs, o) : buf_ld2(rs, o);
+          R.v[t][j] = HD == 128 ? __builtin_amdgcn_raw_buffer_load_b32(rs, vo + j * RB, so, 0)
+                                : (uint32_t)__builtin_amdgcn_raw_buffer_load_b16(rs, vo + j * RB, so, 0);
         }
       }
       if constexpr (BITS == 4) {
-        const uint32_t o = r < r1 ? a.page * RB + slot * (HD / 32) : BUF_OOB;
-        if constexpr (HD == 128) R.vs[t] = buf_ld16(rs, o);
-        else R.vs[t] = buf_ld8(rs, o);
+        if constexpr (HD == 128) R.vs[t] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(rs, vso, ss, 0));
+        else R.vs[t] = __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(rs, vso, ss, 0));
       }
     }
   };
@@ -136,8 +226,8 @@ __global__ __launch_bounds__(PS_THREADS, 2) void k_paged_split(ThvmPagedArgs a, 
     const int32_t id = ids(0);
     idn = ids(1);
     place(id, 0);
-    issue_k(0);
-    issue_v(0);
+    issue_k();
+    issue_v();
   }
   for (int it = 0; it < nt; it++) {
     f32x4_t sc[4];
@@ -158,23 +248,19 @@ __global__ __launch_bounds__(PS_THREADS, 2) void k_paged_split(ThvmPagedArgs a, 
         }
       }
     }
-    bool has[4];                                           // tiles with a page
+    uint32_t has = 0;                                      // tiles with a page
 #pragma unroll
-    for (int t = 0; t < 4; t++) has[t] = rng[t] != 0;
-    uint64_t voff[4];
-#pragma unroll
-    for (int t = 0; t < 4; t++) voff[t] = off[t];
+    for (int t = 0; t < 4; t++) has |= T[t].rows ? 1u << t : 0u;
     // this lane's scores: tile s NG + lc / CG of set s
     float p[NS][4];
     float mx = -INFINITY;
 #pragma unroll
     for (int s = 0; s < NS; s++) {
       f32x4_t v = sc[s * NG];
-      bool ok = has[s * NG];
 #pragma unroll
-      for (int j = 1; j < NG; j++) {
-        if (lc / CG == j) { v = sc[s * NG + j]; ok = has[s * NG + j]; }
-      }
+      for (int j = 1; j < NG; j++)
+        if (lc / CG == j) v = sc[s * NG + j];
+      const bool ok = has >> (s * NG + lc / CG) & 1;
       const int32_t rb = row_of(it, s * NG + lc / CG) + 4 * lg;
 #pragma unroll
       for (int i = 0; i < 4; i++) {
@@ -207,10 +293,9 @@ __global__ __launch_bounds__(PS_THREADS, 2) void k_paged_split(ThvmPagedArgs a, 
         for (int i = 0; i < 4; i++) acc[e][i] *= f;
     }
     // the next step's K while this one's V is used
-    const bool more = it + 1 < nt;
-    place(more ? idn : -1, it + 1);
+    place(idn, it + 1);
     idn = ids(it + 2);
-    issue_k(it + 1);
+    issue_k();
     // V: 16-bit values of rows 4 lg + j, columns EC lc ..
     uint32_t w[4][4][EC / 2];
     bool odd = false;                                      // a value that is not finite
@@ -229,7 +314,7 @@ __global__ __launch_bounds__(PS_THREADS, 2) void k_paged_split(ThvmPagedArgs a, 
           else sb = ((const uint32_t *)&R.vs[t])[j / 2] >> (16 * (j & 1) + 8 * (lc / 8)) & 0xffu;
           if (rt + 16 > first) {                           // wave-uniform: rows that some column does not see, or none
             if (rt + 4 * lg + j >= r1) sb = 0;
-            if (sb == 255u) { odd = true; sb = 0; R.v[t][j] = 0; }
+            odd |= sb == 255u;
           }
           const float f = e8m0_f(sb);
           w[t][j][0] = fp4x2<XT, 0>(R.v[t][j], f);
@@ -253,11 +338,23 @@ __global__ __launch_bounds__(PS_THREADS, 2) void k_paged_split(ThvmPagedArgs a, 
             big = __builtin_elementwise_max(big, __builtin_bit_cast(u16x2, w[t][j][e] & (EXP | EXP << 16)));
       odd = big[0] == EXP || big[1] == EXP;
     }
-    // A zero p times a V that is not finite is NaN: such values (a stored overflow;
-    // a 4-bit group that held one) leave the products, and the columns that see
-    // their rows add them one by one.
-    const bool fix = __builtin_amdgcn_ballot_w64(odd) != 0;
-    if (fix && BITS == 16) {
+    // tiles 2h and 2h + 1: the P operand from its terms, V^T's for column EC lc + e
+    auto pair = [&](int h, const uint32_t (*x)[2]) {
+      const int s0 = (2 * h) / NG, g0 = (2 * h) % NG, s1 = (2 * h + 1) / NG, g1 = (2 * h + 1) % NG;
+      const bool in0 = NG == 1 || lc / CG == g0, in1 = NG == 1 || lc / CG == g1;
+      return make_uint4(in0 ? x[s0][0] : 0u, in0 ? x[s0][1] : 0u, in1 ? x[s1][0] : 0u, in1 ? x[s1][1] : 0u);
+    };
+    auto vt = [&](int h, int e) {
+      const uint32_t sel = (e & 1) ? 0x07060302u : 0x05040100u;
+      return make_uint4(__builtin_amdgcn_perm(w[2 * h][1][e >> 1], w[2 * h][0][e >> 1], sel),
+                        __builtin_amdgcn_perm(w[2 * h][3][e >> 1], w[2 * h][2][e >> 1], sel),
+                        __builtin_amdgcn_perm(w[2 * h + 1][1][e >> 1], w[2 * h + 1][0][e >> 1], sel),
+                        __builtin_amdgcn_perm(w[2 * h + 1][3][e >> 1], w[2 * h + 1][2][e >> 1], sel));
+    };
+    // A zero p times a V that is not finite is NaN: such values (a stored overflow; a
+    // 4-bit group that held one) leave the products, and the columns that see their
+    // rows add them one by one, over the sums in LDS.
+    if (__builtin_amdgcn_ballot_w64(odd)) {                // wave-uniform
 #pragma unroll
       for (int t = 0; t < 4; t++)
 #pragma unroll
@@ -267,63 +364,54 @@ __global__ __launch_bounds__(PS_THREADS, 2) void k_paged_split(ThvmPagedArgs a, 
             if ((w[t][j][e] & EXP) == EXP) w[t][j][e] &= 0xffff0000u;
             if ((w[t][j][e] >> 16 & EXP) == EXP) w[t][j][e] &= 0xffffu;
           }
-    }
+      float *const mine = &wacc[wv][lc][4 * EC * lg];      // d = EC (4 lg + i) + e
 #pragma unroll
-    for (int h = 0; h < 2; h++) {                          // tiles 2h and 2h + 1
-      const int s0 = (2 * h) / NG, g0 = (2 * h) % NG, s1 = (2 * h + 1) / NG, g1 = (2 * h + 1) % NG;
-      const bool in0 = NG == 1 || lc / CG == g0, in1 = NG == 1 || lc / CG == g1;
-      const uint4 B = make_uint4(in0 ? pk[s0][0] : 0u, in0 ? pk[s0][1] : 0u, in1 ? pk[s1][0] : 0u, in1 ? pk[s1][1] : 0u);
-      const uint4 B2 = make_uint4(in0 ? pl2[s0][0] : 0u, in0 ? pl2[s0][1] : 0u, in1 ? pl2[s1][0] : 0u, in1 ? pl2[s1][1] : 0u);
+      for (int i = 0; i < 4; i++)
 #pragma unroll
-      for (int e = 0; e < EC; e++) {
-        const uint32_t sel = (e & 1) ? 0x07060302u : 0x05040100u;
-        uint4 A;
-        A.x = __builtin_amdgcn_perm(w[2 * h][1][e >> 1], w[2 * h][0][e >> 1], sel);
-        A.y = __builtin_amdgcn_perm(w[2 * h][3][e >> 1], w[2 * h][2][e >> 1], sel);
-        A.z = __builtin_amdgcn_perm(w[2 * h + 1][1][e >> 1], w[2 * h + 1][0][e >> 1], sel);
-        A.w = __builtin_amdgcn_perm(w[2 * h + 1][3][e >> 1], w[2 * h + 1][2][e >> 1], sel);
-        acc[e] = mfma16<XT>(A, B, acc[e]);
-        acc[e] = mfma16<XT>(A, B2, acc[e]);
-      }
-    }
-    if (fix) {                                             // wave-uniform
+        for (int e = 0; e < EC; e++) mine[EC * i + e] = acc[e][i];
 #pragma unroll
       for (int s = 0; s < NS; s++) {
-        uint64_t vo = voff[s * NG];
-        bool ok = has[s * NG];
-#pragma unroll
-        for (int j = 1; j < NG; j++)
-          if (lc / CG == j) { vo = voff[s * NG + j]; ok = has[s * NG + j]; }
         const int32_t rt = row_of(it, s * NG + lc / CG);
-        const char *vb = (const char *)a.vpages + vo;
 #pragma unroll 1
         for (int jj = 0; jj < 4; jj++)
 #pragma unroll
           for (int i = 0; i < 4; i++) {
             const float pr = __shfl(p[s][i], lc + 16 * jj);
-            const int32_t r = rt + 4 * jj + i;
-            if (!ok || r >= lim) continue;
+            const int32_t r = rt + 4 * jj + i, id = r < lim ? pg_page(&a, u.s, r) : -1;
+            if (id < 0) continue;
+            const char *vb = (const char *)a.vpages + pg_block(&a, id, kvh);
             const uint32_t slot = (uint32_t)r & pm;
-#pragma unroll
-            for (int q = 0; q < 4; q++)                    // this lane's d = EC (4 lg + q) + e
-#pragma unroll
-              for (int e = 0; e < EC; e++) {
-                const uint32_t d = EC * (4 * lg + q) + e;
-                float x;
-                if constexpr (BITS == 16) {
-                  const uint32_t h = ((const uint16_t *)vb)[slot * HD + d];
-                  if ((h & EXP) != EXP) continue;
-                  x = P::lo(h);
-                } else {
-                  if ((uint8_t)vb[a.page * RB + slot * (HD / 32) + d / 32] != 255u) continue;
-                  x = __builtin_nanf("");
-                }
-                acc[e][q] += pr * x;
+#pragma unroll 1
+            for (int k = 0; k < 4 * EC; k++) {
+              const uint32_t d = 4 * EC * lg + k;
+              float x = __builtin_nanf("");
+              if (BITS == 16) {
+                const uint32_t h = ((const uint16_t *)vb)[slot * HD + d];
+                if ((h & EXP) != EXP) continue;
+                x = P::lo(h);
+              } else if ((uint8_t)vb[a.page * RB + slot * (HD / 32) + d / 32] != 255u) {
+                continue;
               }
+              mine[k] += pr * x;
+            }
           }
       }
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+#pragma unroll
+        for (int e = 0; e < EC; e++) acc[e][i] = mine[EC * i + e];
     }
-    issue_v(it + 1);
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+      const uint4 B = pair(h, pk), B2 = pair(h, pl2);
+#pragma unroll
+      for (int e = 0; e < EC; e++) {
+        const uint4 A = vt(h, e);
+        acc[e] = mfma16<XT>(A, B, acc[e]);
+        acc[e] = mfma16<XT>(A, B2, acc[e]);
+      }
+    }
+    issue_v();
   }
   // the waves (and the column groups) meet in LDS
   l += xor16_f(l);
@@ -355,68 +443,42 @@ __global__ __launch_bounds__(PS_THREADS, 2) void k_paged_split(ThvmPagedArgs a, 
       const float inv = lt != 0.0f ? 1.0f / lt : 0.0f;
       *(uint32_t *)((uint16_t *)a.out + ((uint64_t)(u.q.r0 + cc / G) * a.H + kvh * G + cc % G) * HD + d) = P::pk(s0 * inv, s1 * inv);
     } else {
-      float *pp = a.ws + (((uint64_t)kvh * pl.units + un) * CG + c) * (HD + 4);
-      *(float2 *)(pp + d) = make_float2(s0, s1);
-      if (d == 0) *(float2 *)(pp + HD) = make_float2(M, lt);
+      float *const rec = a.ws + ((uint64_t)kvh * pl.units + un) * CG * (HD + 4), *pp = rec + c * (HD + 4);
+      if (pl.fuse) {
+        coh_st8(rec, (c * (HD + 4) + d) * 4, make_uint2(__float_as_uint(s0), __float_as_uint(s1)));
+        if (d == 0) coh_st8(rec, (c * (HD + 4) + HD) * 4, make_uint2(__float_as_uint(M), __float_as_uint(lt)));
+      } else {
+        *(float2 *)(pp + d) = make_float2(s0, s1);
+        if (d == 0) *(float2 *)(pp + HD) = make_float2(M, lt);
+      }
     }
   }
+  if (u.nchunk == 1 || !pl.fuse) return;
+  // the tile's last block adds the chunks up, in chunk order
+  __shared__ uint32_t lastf;
+  vm_drain();
+  __syncthreads();
+  if (tid == 0) {
+    uint32_t *ctr = pa_arrived + (uint64_t)kvh * pl.units + u.first;
+    const uint32_t old = __hip_atomic_fetch_add(ctr, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    lastf = old == u.nchunk - 1 ? 1u : 0u;
+    if (lastf) __hip_atomic_exchange(ctr, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  __syncthreads();
+  if (!lastf) return;                                      // block-uniform
+  pa_fold<HD, XT, CG, (1024 / HD) / CG ? (1024 / HD) / CG : 1, true>(
+      a, pl, u, kvh, (float4(*)[HD / 4])&wacc[0][0][0], &wm[0][0], &wl[0][0]);
 }
 
-// k_paged_merge: the chunks of a column, their partials (sum, m, l) in a fixed
-// order.  HD / 4 lanes take a chunk; NP such groups take every NP-th chunk of one
-// column and meet in LDS, the block's other groups have other columns.
+// k_paged_merge: the chunks of the tiles that have several, in a launch of its own.
 template <int HD, int XT, int CT, int NP>
 __global__ __launch_bounds__(256) void k_paged_merge(ThvmPagedArgs a, PgPlan pl) {
-  typedef PgT<XT> P;
-  constexpr int LN = HD / 4, NG = 256 / LN, CB = NG / NP;  // lanes a chunk, groups, columns a block
-  __shared__ float4 ls[NG][LN];
-  __shared__ float lm[NG], ll[NG];
-  const uint32_t g = threadIdx.x / LN, x = threadIdx.x % LN, part = g % NP;
-  const uint32_t c = blockIdx.x % (CT / CB) * CB + g / NP, kvh = blockIdx.x / (CT / CB) % a.Hkv, G = a.H / a.Hkv;
+  constexpr int CB = 1024 / HD / NP;                       // columns a block
+  __shared__ float4 ls[1024 / HD][HD / 4];
+  __shared__ float lm[1024 / HD], ll[1024 / HD];
   PgUnit u;
   if (!pg_unit(a, pl, blockIdx.x / (CT / CB) / a.Hkv, true, u) || u.nchunk == 1) return;
-  const uint32_t cc = u.tile * pl.ct + c;
-  const bool live = (int32_t)(cc / G) < u.q.r1 - u.q.r0;
-  const float *pp = a.ws + (((uint64_t)kvh * pl.units + u.first) * CT + c) * (HD + 4);
-  const uint64_t st = (uint64_t)CT * (HD + 4);
-  float m = -INFINITY, l = 0.0f;
-  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (uint32_t k = part; live && k < u.nchunk; k += NP) {
-    const float4 w = *(const float4 *)(pp + k * st + 4 * x);
-    const float2 ml = *(const float2 *)(pp + k * st + HD);
-    const float mn = fmaxf(m, ml.x), f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn),
-                e = ml.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(ml.x - mn);
-    v.x = v.x * f + w.x * e;
-    v.y = v.y * f + w.y * e;
-    v.z = v.z * f + w.z * e;
-    v.w = v.w * f + w.w * e;
-    l = l * f + ml.y * e;
-    m = mn;
-  }
-  if (NP > 1) {
-    ls[g][x] = v;
-    if (x == 0) { lm[g] = m; ll[g] = l; }
-    __syncthreads();
-    if (part) return;
-    float M = -INFINITY;
-#pragma unroll
-    for (int k = 0; k < NP; k++) M = fmaxf(M, lm[g + k]);
-    l = 0.0f;
-    v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-    for (int k = 0; k < NP; k++) {
-      const float f = lm[g + k] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(lm[g + k] - M);
-      v.x += ls[g + k][x].x * f;
-      v.y += ls[g + k][x].y * f;
-      v.z += ls[g + k][x].z * f;
-      v.w += ls[g + k][x].w * f;
-      l += ll[g + k] * f;
-    }
-  }
-  if (!live) return;
-  const float inv = l != 0.0f ? 1.0f / l : 0.0f;
-  *(uint2 *)((uint16_t *)a.out + ((uint64_t)(u.q.r0 + cc / G) * a.H + kvh * G + cc % G) * HD + 4 * x) =
-      make_uint2(P::pk(v.x * inv, v.y * inv), P::pk(v.z * inv, v.w * inv));
+  pa_fold<HD, XT, CT, NP, false>(a, pl, u, blockIdx.x / (CT / CB) % a.Hkv, ls, lm, ll, blockIdx.x % (CT / CB) * CB);
 }
 
 // ---- which kernels a call takes ------------------------------------------------
@@ -433,11 +495,16 @@ static PaRule pa_rule(const ThvmPagedArgs *a) {
   r.many = most > hi;
   r.few = !r.many || a->ragged;
   r.few_tiles = a->b * ((hi + 15) / 16);
-  r.fpl = PgPlan{0, hi, 16, fill > 2 * r.few_tiles ? fill : 2 * r.few_tiles, 1, 0};
+  r.fpl = PgPlan{0, hi, 16, fill > 2 * r.few_tiles ? fill : 2 * r.few_tiles, 4, 0, 0};
+  // about as many chunks as a tile can have, twice the mean where the units are shared
+  const uint64_t cap = ((uint64_t)a->maxpages * a->page + 64 * r.fpl.cmin - 1) / (64 * r.fpl.cmin), mean = 2 * r.fpl.units / r.few_tiles + 1;
+  const uint64_t chunks = cap < mean ? cap : mean < r.fpl.units ? mean : r.fpl.units;
+  r.fpl.fuse = chunks * r.cg <= 96 && (uint64_t)a->Hkv * r.fpl.units <= PA_COUNTERS &&
+               (uint64_t)r.fpl.units * r.cg * (a->hd + 4) * 4 < (1ull << 31);
   const uint32_t whole = (uint32_t)((uint64_t)a->n * G / PP_COLS);
   r.many_tiles = whole + a->b;
   r.split = (uint64_t)whole * a->Hkv < 512;
-  r.mpl = PgPlan{r.few ? hi : 0, 0xffffffffu, PP_COLS, r.many_tiles + 1, 1u << 25, 1};
+  r.mpl = PgPlan{r.few ? hi : 0, 0xffffffffu, PP_COLS, r.many_tiles + 1, 1u << 25, 1, 0};
   if (r.split) {
     r.mpl.units = fill > 2 * r.many_tiles ? fill : 2 * r.many_tiles;
     r.mpl.cmin = 4;
@@ -472,8 +539,10 @@ extern "C" int thvm_k_attn_paged(const ThvmPagedArgs *a, hipStream_t s, char *er
   const PaKernels k = a->hd == 128 ? (bf ? pa_pick<128, GX_BF16>(a, r.cg) : pa_pick<128, GX_F16>(a, r.cg))
                                    : (bf ? pa_pick<64, GX_BF16>(a, r.cg) : pa_pick<64, GX_F16>(a, r.cg));
   if (r.few) {
-    thvm_launch(true, false, k.split, dim3(a->Hkv * r.fpl.units), dim3(PS_THREADS), 0, s, *a, r.fpl);
-    thvm_launch(false, !r.many, k.merge, dim3(a->Hkv * r.cg * r.few_tiles), dim3(256), 0, s, *a, r.fpl);
+    const bool last = !r.many;
+    thvm_launch(true, last && r.fpl.fuse, k.split, dim3(a->Hkv * r.fpl.units), dim3(PS_THREADS), 0, s, *a, r.fpl);
+    if (!r.fpl.fuse)
+      thvm_launch(false, last, k.merge, dim3(a->Hkv * r.cg * r.few_tiles), dim3(256), 0, s, *a, r.fpl);
   }
   if (r.many) {
     thvm_launch(!r.few, !r.split, pp_tile_pick(a), dim3(a->Hkv * r.mpl.units), dim3(PP_THREADS), 0, s, *a, r.mpl);

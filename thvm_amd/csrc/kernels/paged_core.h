@@ -67,6 +67,8 @@ __device__ __forceinline__ uint32_t fp4x2(uint32_t w, float scale) {
 }
 __device__ __forceinline__ float e8m0_f(uint32_t byte) { return __uint_as_float(byte << 23); }
 
+template <bool V> struct pg_const { static constexpr bool value = V; };
+
 // ---- units of work -----------------------------------------------------------
 // A kernel takes the sequences whose columns (rows x the G query heads of a kv
 // head) number more than lo and at most hi, ct columns a tile, and splits each
@@ -77,7 +79,7 @@ __device__ __forceinline__ float e8m0_f(uint32_t byte) { return __uint_as_float(
 // try always does (a tile adds one chunk at most to its share); the host launches
 // units >= 2 x tiles, so c never passes the mean length of the tiles: long
 // sequences are split, short ones are not, and the blocks are of one size.
-struct PgPlan { uint32_t lo, hi, ct, units, cmin, rev; };
+struct PgPlan { uint32_t lo, hi, ct, units, cmin, rev, fuse; };
 struct PgUnit { PgSeq q; uint32_t s, tile, chunk, nchunk, c, first, u; };
 
 __device__ __forceinline__ float wave_scan(float v) {           // inclusive, lane order

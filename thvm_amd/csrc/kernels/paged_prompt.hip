@@ -44,8 +44,6 @@ __device__ __forceinline__ void buf_lds16(buf_t r, char *dst, uint32_t off) {
 #endif
 }
 
-template <bool V> struct pp_const { static constexpr bool value = V; };
-
 // byte of 16-byte piece c of row r in a step's K or V
 template <int HD> __device__ __forceinline__ uint32_t k_at(uint32_t r, uint32_t c) {
   return r * (HD * 2) + ((c ^ (HD == 128 ? r & 15u : r >> 1 & 7u)) << 4);
@@ -365,15 +363,15 @@ __global__ __launch_bounds__(PP_THREADS, 2) void k_paged_tile(ThvmPagedArgs a, P
   };
   if (nt) {
     scores(lk0, S0);
-    move(top(pp_const<true>{}, 0, holes_of(i0), S0));
+    move(top(pg_const<true>{}, 0, holes_of(i0), S0));
   }
   while (j + 2 < nt && full(i0, j) && full(i1, j + 1) && full(i2, j + 2)) {
-    step(pp_const<false>{}, S0, S1, lk0, lk1, lv0, lv1);
-    step(pp_const<false>{}, S1, S0, lk1, lk0, lv1, lv0);
+    step(pg_const<false>{}, S0, S1, lk0, lk1, lv0, lv1);
+    step(pg_const<false>{}, S1, S0, lk1, lk0, lv1, lv0);
   }
   while (j < nt) {
-    step(pp_const<true>{}, S0, S1, lk0, lk1, lv0, lv1);
-    if (j < nt) step(pp_const<true>{}, S1, S0, lk1, lk0, lv1, lv0);
+    step(pg_const<true>{}, S0, S1, lk0, lk1, lv0, lv1);
+    if (j < nt) step(pg_const<true>{}, S1, S0, lk1, lk0, lv1, lv0);
   }
   if (!live) return;
   l += xor32_f(l);
