@@ -14,18 +14,17 @@
 
 // Columns of a tile from their chunks' partials (sum, m, l), in a fixed order.  HD /
 // 4 lanes take a chunk; NP such groups of a block take every NP-th chunk of one
-// column and meet in LDS, its other groups have other columns, from c0 on and (all
-// of the tile's CT, COH) in rounds.  COH: partials of blocks of this launch, read past
-// the caches.
+// column and meet in LDS, its other groups have other columns; columns c0 to c1, in
+// rounds.  COH: partials of blocks of this launch, read past the caches.
 template <int HD, int XT, int CT, int NP, bool COH>
 __device__ __forceinline__ void pa_fold(const ThvmPagedArgs &a, const PgPlan &pl, const PgUnit &u, uint32_t kvh,
-                                        float4 (*ls)[HD / 4], float *lm, float *ll, uint32_t c0 = 0) {
+                                        float4 (*ls)[HD / 4], float *lm, float *ll, uint32_t c0, uint32_t c1) {
   typedef PgT<XT> P;
   constexpr int LN = HD / 4, NG = 256 / LN, CB = NG / NP, BT = 8;   // lanes a chunk, groups, columns at once, loads ahead
   const uint32_t g = threadIdx.x / LN, x = threadIdx.x % LN, part = g % NP, G = a.H / a.Hkv;
   const uint64_t st = (uint64_t)CT * (HD + 4);
   const float *const base = a.ws + ((uint64_t)kvh * pl.units + u.first) * st;
-  for (uint32_t c = c0 + g / NP; c < (COH ? (uint32_t)CT : c0 + CB); c += CB) {   // (as many rounds for every thread)
+  for (uint32_t c = c0 + g / NP; c < c1; c += CB) {        // (as many rounds for every thread)
     const uint32_t cc = u.tile * pl.ct + c;
     const bool live = (int32_t)(cc / G) < u.q.r1 - u.q.r0;
     const float *pp = base + (uint64_t)c * (HD + 4);
@@ -443,7 +442,7 @@ __global__ __launch_bounds__(PS_THREADS, 2) void k_paged_split(ThvmPagedArgs a, 
       const float inv = lt != 0.0f ? 1.0f / lt : 0.0f;
       *(uint32_t *)((uint16_t *)a.out + ((uint64_t)(u.q.r0 + cc / G) * a.H + kvh * G + cc % G) * HD + d) = P::pk(s0 * inv, s1 * inv);
     } else {
-      float *const rec = a.ws + ((uint64_t)kvh * pl.units + un) * CG * (HD + 4), *pp = rec + c * (HD + 4);
+      float *const rec = a.ws + ((uint64_t)kvh * pl.units + u.u) * CG * (HD + 4), *pp = rec + c * (HD + 4);
       if (pl.fuse) {
         coh_st8(rec, (c * (HD + 4) + d) * 4, make_uint2(__float_as_uint(s0), __float_as_uint(s1)));
         if (d == 0) coh_st8(rec, (c * (HD + 4) + HD) * 4, make_uint2(__float_as_uint(M), __float_as_uint(lt)));
@@ -467,18 +466,21 @@ __global__ __launch_bounds__(PS_THREADS, 2) void k_paged_split(ThvmPagedArgs a, 
   __syncthreads();
   if (!lastf) return;                                      // block-uniform
   pa_fold<HD, XT, CG, (1024 / HD) / CG ? (1024 / HD) / CG : 1, true>(
-      a, pl, u, kvh, (float4(*)[HD / 4])&wacc[0][0][0], &wm[0][0], &wl[0][0]);
+      a, pl, u, kvh, (float4(*)[HD / 4])&wacc[0][0][0], &wm[0][0], &wl[0][0], 0, CG);
 }
 
-// k_paged_merge: the chunks of the tiles that have several, in a launch of its own.
-template <int HD, int XT, int CT, int NP>
+#define PA_MERGE 32                                        // columns a block of a prompt tile's merge
+
+// k_paged_merge: the chunks of the tiles that have several, in a launch of its own, CB
+// columns a block.
+template <int HD, int XT, int CT, int NP, int CB>
 __global__ __launch_bounds__(256) void k_paged_merge(ThvmPagedArgs a, PgPlan pl) {
-  constexpr int CB = 1024 / HD / NP;                       // columns a block
   __shared__ float4 ls[1024 / HD][HD / 4];
   __shared__ float lm[1024 / HD], ll[1024 / HD];
   PgUnit u;
   if (!pg_unit(a, pl, blockIdx.x / (CT / CB) / a.Hkv, true, u) || u.nchunk == 1) return;
-  pa_fold<HD, XT, CT, NP, false>(a, pl, u, blockIdx.x / (CT / CB) % a.Hkv, ls, lm, ll, blockIdx.x % (CT / CB) * CB);
+  const uint32_t c0 = blockIdx.x % (CT / CB) * CB;
+  pa_fold<HD, XT, CT, NP, false>(a, pl, u, blockIdx.x / (CT / CB) % a.Hkv, ls, lm, ll, c0, c0 + CB);
 }
 
 // ---- which kernels a call takes ------------------------------------------------
@@ -495,7 +497,7 @@ static PaRule pa_rule(const ThvmPagedArgs *a) {
   r.many = most > hi;
   r.few = !r.many || a->ragged;
   r.few_tiles = a->b * ((hi + 15) / 16);
-  r.fpl = PgPlan{0, hi, 16, fill > 2 * r.few_tiles ? fill : 2 * r.few_tiles, 4, 0, 0};
+  r.fpl = PgPlan{0, hi, 16, fill > 2 * r.few_tiles ? fill : 2 * r.few_tiles, 4, 0};
   // about as many chunks as a tile can have, twice the mean where the units are shared
   const uint64_t cap = ((uint64_t)a->maxpages * a->page + 64 * r.fpl.cmin - 1) / (64 * r.fpl.cmin), mean = 2 * r.fpl.units / r.few_tiles + 1;
   const uint64_t chunks = cap < mean ? cap : mean < r.fpl.units ? mean : r.fpl.units;
@@ -504,7 +506,7 @@ static PaRule pa_rule(const ThvmPagedArgs *a) {
   const uint32_t whole = (uint32_t)((uint64_t)a->n * G / PP_COLS);
   r.many_tiles = whole + a->b;
   r.split = (uint64_t)whole * a->Hkv < 512;
-  r.mpl = PgPlan{r.few ? hi : 0, 0xffffffffu, PP_COLS, r.many_tiles + 1, 1u << 25, 1, 0};
+  r.mpl = PgPlan{r.few ? hi : 0, 0xffffffffu, PP_COLS, r.many_tiles + 1, 1u << 25, 0};
   if (r.split) {
     r.mpl.units = fill > 2 * r.many_tiles ? fill : 2 * r.many_tiles;
     r.mpl.cmin = 4;
@@ -528,8 +530,8 @@ template <int HD, int XT>
 static PaKernels pa_pick(const ThvmPagedArgs *a, uint32_t cg) {
   constexpr int NG = 1024 / HD;                            // one column a block
   return PaKernels{a->bits == 16 ? pa_split<HD, XT, 16>(cg) : pa_split<HD, XT, 4>(cg),
-                   cg == 4 ? k_paged_merge<HD, XT, 4, NG> : cg == 8 ? k_paged_merge<HD, XT, 8, NG> : k_paged_merge<HD, XT, 16, NG>,
-                   k_paged_merge<HD, XT, PP_COLS, 2>};
+                   cg == 4 ? k_paged_merge<HD, XT, 4, NG, 1> : cg == 8 ? k_paged_merge<HD, XT, 8, NG, 1> : k_paged_merge<HD, XT, 16, NG, 1>,
+                   k_paged_merge<HD, XT, PP_COLS, 1, PA_MERGE>};
 }
 
 extern "C" int thvm_k_attn_paged(const ThvmPagedArgs *a, hipStream_t s, char *err, int errlen) {
@@ -546,10 +548,8 @@ extern "C" int thvm_k_attn_paged(const ThvmPagedArgs *a, hipStream_t s, char *er
   }
   if (r.many) {
     thvm_launch(!r.few, !r.split, pp_tile_pick(a), dim3(a->Hkv * r.mpl.units), dim3(PP_THREADS), 0, s, *a, r.mpl);
-    if (r.split) {
-      const uint32_t cb = 256 / (a->hd / 4) / 2;           // columns a block
-      thvm_launch(false, true, k.tmerge, dim3(a->Hkv * (PP_COLS / cb) * r.many_tiles), dim3(256), 0, s, *a, r.mpl);
-    }
+    if (r.split)
+      thvm_launch(false, true, k.tmerge, dim3(a->Hkv * (PP_COLS / PA_MERGE) * r.many_tiles), dim3(256), 0, s, *a, r.mpl);
   }
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) { snprintf(err, errlen, "attn_paged launch: %s", hipGetErrorString(e)); return -1; }

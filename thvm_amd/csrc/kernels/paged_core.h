@@ -78,8 +78,10 @@ template <bool V> struct pg_const { static constexpr bool value = V; };
 // steps / (units - tiles) with which the chunks number at most `units`.  The last
 // try always does (a tile adds one chunk at most to its share); the host launches
 // units >= 2 x tiles, so c never passes the mean length of the tiles: long
-// sequences are split, short ones are not, and the blocks are of one size.
-struct PgPlan { uint32_t lo, hi, ct, units, cmin, rev, fuse; };
+// sequences are split, short ones are not, and the blocks are of one size but for
+// the last chunk of each tile.  Those come after the whole ones.  `fuse`: the last
+// block of a tile adds its chunks.
+struct PgPlan { uint32_t lo, hi, ct, units, cmin, fuse; };
 struct PgUnit { PgSeq q; uint32_t s, tile, chunk, nchunk, c, first, u; };
 
 __device__ __forceinline__ float wave_scan(float v) {           // inclusive, lane order
@@ -133,35 +135,46 @@ __device__ __forceinline__ bool pg_unit(const ThvmPagedArgs &a, const PgPlan &p,
     c = c1 + (uint32_t)((uint64_t)(c2 - c1) * k / 4);
   }
   o.c = c;
-  if (p.rev && !tiles_only) {                                          // a block per unit: the last ones first
-    float n = 0.0f;
-    each([&](uint32_t, const PgSeq &, float t, float l) { n += wave_sum(t * (float)(((uint32_t)l + c - 1) / c)); });
+  // the order of the blocks: whole chunks first, then the tiles' shorter last ones (all
+  // of a tile where none is split: backwards, as a prompt's last tiles see most)
+  uint32_t at = u;
+  bool rest = false;
+  if (!tiles_only) {
+    float whole = 0.0f, n = 0.0f;
+    each([&](uint32_t, const PgSeq &, float t, float l) {
+      whole += wave_sum(t * (float)((uint32_t)l / c));
+      n += wave_sum(t * (float)(((uint32_t)l + c - 1) / c));
+    });
     if ((float)u >= n) return false;
-    u = (uint32_t)n - 1 - u;
+    rest = (float)u >= whole;
+    at = rest ? u - (uint32_t)whole : u;
+    if (whole == 0.0f) at = (uint32_t)n - 1 - u;
   }
-  o.u = u;
-  float before = 0.0f, tbefore = 0.0f;
+  float before = 0.0f, kbefore = 0.0f;
   bool found = false;
   each([&](uint32_t s0, const PgSeq &q, float t, float l) {
     if (found) return;
-    const float per = (float)(((uint32_t)l + c - 1) / c), n = t * per, sc = wave_scan(n), tc = wave_scan(t);
-    const uint64_t hit = __builtin_amdgcn_ballot_w64((tiles_only ? tbefore + tc : before + sc) > (float)u);
+    const float per = (float)(((uint32_t)l + c - 1) / c), full = (float)((uint32_t)l / c), n = t * per;
+    const float key = tiles_only ? t : t * (rest ? per - full : full);
+    const float sc = wave_scan(n), kc = wave_scan(key);
+    const uint64_t hit = __builtin_amdgcn_ballot_w64(kbefore + kc > (float)at);
     if (hit) {
       const int w = __builtin_ctzll(hit);
-      auto at = [&](float v) { return (uint32_t)__int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), w)); };
+      auto get = [&](float v) { return (uint32_t)__int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), w)); };
       found = true;
       o.s = s0 + w;
       o.q.r0 = __builtin_amdgcn_readlane(q.r0, w);
       o.q.r1 = __builtin_amdgcn_readlane(q.r1, w);
       o.q.len = __builtin_amdgcn_readlane(q.len, w);
-      o.nchunk = at(per);
-      const uint32_t first = at(before + sc - n), tfirst = at(tbefore + tc - t);
-      o.tile = tiles_only ? u - tfirst : (u - first) / o.nchunk;
-      o.chunk = tiles_only ? 0 : (u - first) % o.nchunk;
-      o.first = first + o.tile * o.nchunk;
+      o.nchunk = get(per);
+      const uint32_t i = at - get(kbefore + kc - key), f = get(full);
+      o.tile = tiles_only || rest ? i : i / f;
+      o.chunk = tiles_only ? 0 : rest ? f : i % f;
+      o.first = get(before + sc - n) + o.tile * o.nchunk;
+      o.u = o.first + o.chunk;
     }
     before += wave_sum(n);
-    tbefore += wave_sum(t);
+    kbefore += wave_sum(key);
   });
   return found;
 }
