@@ -9,7 +9,7 @@
 // (no contraction): next to a border between two 4-bit codes every order of
 // evaluation then picks the same code.
 //   * a lane owns 8 consecutive values (one 16-byte load), 16 or 8 lanes a head;
-//     a wave takes 4 groups of 4 or 8 heads of ONE row, so its sequence, position,
+//     a wave takes 1 or 4 groups of 4 or 8 heads of ONE row, so its sequence, position,
 //     page and rotation are found once, with all its x already on its way;
 //   * the partner of a half rotation and the 32 values of a 4-bit group lie in
 //     the head's own lanes: no LDS.
@@ -18,7 +18,7 @@
 #include "paged_core.h"
 
 #define PC_THREADS 256
-#define PC_U 4                                          // groups of heads a wave takes
+#define PC_FILL 2048                                    // waves of four groups that fill the card
 
 template <int CTRL>
 __device__ __forceinline__ double dpp_d(double v) {
@@ -32,7 +32,7 @@ __device__ __forceinline__ uint32_t dpp_u(uint32_t v) {
   return __builtin_amdgcn_update_dpp(0, v, CTRL, 0xf, 0xf, true);
 }
 
-// What a wave works on: PC_U groups of heads of one row, the row's sequence and
+// What a wave works on: U groups of heads of one row, the row's sequence and
 // position.
 struct PcRow { uint32_t row, g0; int32_t pos, id; bool ok; };
 __device__ __forceinline__ uint32_t pc_wave() {
@@ -50,19 +50,19 @@ __device__ __forceinline__ PcRow pc_place(const ThvmPagedArgs &a, uint32_t row, 
   return r;
 }
 
-template <int HD, int XT, int BITS>
+template <int HD, int XT, int BITS, int U>
 __global__ __launch_bounds__(PC_THREADS) void k_kv_append(ThvmPagedArgs a) {
 #pragma clang fp contract(off)
   typedef PgT<XT> P;
   constexpr int LPV = HD / 8, VPW = 64 / LPV;          // lanes a head, heads a group
-  const uint32_t heads = a.H + 2 * a.Hkv, grps = (heads + VPW - 1) / VPW, wpr = (grps + PC_U - 1) / PC_U;
-  const uint32_t wid = pc_wave(), row = wid / wpr, g0 = wid % wpr * PC_U, lane = lane_id();
+  const uint32_t heads = a.H + 2 * a.Hkv, grps = (heads + VPW - 1) / VPW, wpr = (grps + U - 1) / U;
+  const uint32_t wid = pc_wave(), row = wid / wpr, g0 = wid % wpr * U, lane = lane_id();
   if (row >= a.n) return;
   // x on its way while the row is placed
   const uint32_t d0 = lane % LPV * 8, h0 = g0 * VPW + lane / LPV;
-  uint4 x[PC_U];
+  uint4 x[U];
 #pragma unroll
-  for (int u = 0; u < PC_U; u++) {
+  for (int u = 0; u < U; u++) {
     const uint32_t hv = h0 + u * VPW;
     x[u] = hv < heads ? ld_stream16((const uint16_t *)a.x + (uint64_t)row * a.ldx + hv * HD + d0) : make_uint4(0, 0, 0, 0);
   }
@@ -82,13 +82,13 @@ __global__ __launch_bounds__(PC_THREADS) void k_kv_append(ThvmPagedArgs a) {
       sn[k] = ss.x; sn[k + 1] = ss.y; sn[k + 2] = ss.z; sn[k + 3] = ss.w;
     }
   }
-  float inv[PC_U];
+  float inv[U];
   if (a.norm) {
     // each lane has its head's sums of all groups: it takes one of them through the
-    // root (v_rsq_f64 and two steps of Newton's iteration), and the quad shares out
+    // root (v_rsq_f64 and two steps of Newton's iteration), and a quad shares out four
     double one = 0.0;
 #pragma unroll
-    for (int u = 0; u < PC_U; u++) {
+    for (int u = 0; u < U; u++) {
       const uint32_t w[4] = {x[u].x, x[u].y, x[u].z, x[u].w};
       double ss = 0.0;
 #pragma unroll
@@ -101,21 +101,25 @@ __global__ __launch_bounds__(PC_THREADS) void k_kv_append(ThvmPagedArgs a) {
       ss += dpp_d<0x4E>(ss);
       ss += dpp_d<0x141>(ss);
       if (LPV == 16) ss += dpp_d<0x140>(ss);
-      if ((lane & 3) == u) one = ss;
+      if (U == 1 || (lane & 3) == u) one = ss;
     }
     one = one * (1.0 / HD) + (double)a.eps;
     double y = __builtin_amdgcn_rsq(one);
     y = __builtin_fma(y, __builtin_fma(-0.5 * one * y, y, 0.5), y);
     y = __builtin_fma(y, __builtin_fma(-0.5 * one * y, y, 0.5), y);
     const float f = one == 0.0 ? INFINITY : one == __builtin_inf() ? 0.0f : (float)y;
-    inv[0] = dpp_f<0x00>(f);
-    inv[1] = dpp_f<0x55>(f);
-    inv[2] = dpp_f<0xAA>(f);
-    inv[3] = dpp_f<0xFF>(f);
+    if (U == 1) {
+      inv[0] = f;
+    } else {
+      inv[0] = dpp_f<0x00>(f);
+      inv[1 % U] = dpp_f<0x55>(f);
+      inv[2 % U] = dpp_f<0xAA>(f);
+      inv[3 % U] = dpp_f<0xFF>(f);
+    }
   }
   const uint32_t slot = (uint32_t)r.pos & (a.page - 1);
 #pragma unroll
-  for (int u = 0; u < PC_U; u++) {
+  for (int u = 0; u < U; u++) {
     const uint32_t hv = h0 + u * VPW;
     const bool live = hv < heads, isq = hv < a.H, isv = hv >= a.H + a.Hkv;
     const uint32_t xw[4] = {x[u].x, x[u].y, x[u].z, x[u].w};
@@ -176,19 +180,19 @@ __global__ __launch_bounds__(PC_THREADS) void k_kv_append(ThvmPagedArgs a) {
   }
 }
 
-template <int HD, int XT, int BITS>
+template <int HD, int XT, int BITS, int U>
 __global__ __launch_bounds__(PC_THREADS) void k_kv_read(ThvmPagedArgs a) {
   constexpr int LPV = HD / 8, VPW = 64 / LPV;
-  const uint32_t heads = 2 * a.Hkv, grps = (heads + VPW - 1) / VPW, wpr = (grps + PC_U - 1) / PC_U;
+  const uint32_t heads = 2 * a.Hkv, grps = (heads + VPW - 1) / VPW, wpr = (grps + U - 1) / U;
   const uint32_t wid = pc_wave(), row = wid / wpr, lane = lane_id();
   if (row >= a.n) return;
-  const PcRow r = pc_place(a, row, wid % wpr * PC_U);
+  const PcRow r = pc_place(a, row, wid % wpr * U);
   if (!r.ok) return;
   const uint32_t d0 = lane % LPV * 8, h0 = r.g0 * VPW + lane / LPV, slot = (uint32_t)r.pos & (a.page - 1);
-  uint4 w[PC_U];
-  uint32_t sc[PC_U];
+  uint4 w[U];
+  uint32_t sc[U];
 #pragma unroll
-  for (int u = 0; u < PC_U; u++) {
+  for (int u = 0; u < U; u++) {
     const uint32_t hv = h0 + u * VPW, kvh = hv < a.Hkv ? hv : hv - a.Hkv;
     w[u] = make_uint4(0, 0, 0, 0);
     sc[u] = 0;
@@ -203,7 +207,7 @@ __global__ __launch_bounds__(PC_THREADS) void k_kv_read(ThvmPagedArgs a) {
     }
   }
 #pragma unroll
-  for (int u = 0; u < PC_U; u++) {
+  for (int u = 0; u < U; u++) {
     const uint32_t hv = h0 + u * VPW, kvh = hv < a.Hkv ? hv : hv - a.Hkv;
     if (hv >= heads) continue;
     if (BITS == 4) {
@@ -216,15 +220,25 @@ __global__ __launch_bounds__(PC_THREADS) void k_kv_read(ThvmPagedArgs a) {
 }
 
 typedef void (*pc_fn)(ThvmPagedArgs);
-#define PC_PICK(K) (a->hd == 128 ? (bf ? (a->bits == 16 ? K<128, GX_BF16, 16> : K<128, GX_BF16, 4>)          \
-                                       : (a->bits == 16 ? K<128, GX_F16, 16> : K<128, GX_F16, 4>))          \
-                                 : (bf ? (a->bits == 16 ? K<64, GX_BF16, 16> : K<64, GX_BF16, 4>)            \
-                                       : (a->bits == 16 ? K<64, GX_F16, 16> : K<64, GX_F16, 4>)))
+#define PC_PICK_U(K, U) (a->hd == 128 ? (bf ? (a->bits == 16 ? K<128, GX_BF16, 16, U> : K<128, GX_BF16, 4, U>)   \
+                                            : (a->bits == 16 ? K<128, GX_F16, 16, U> : K<128, GX_F16, 4, U>))   \
+                                      : (bf ? (a->bits == 16 ? K<64, GX_BF16, 16, U> : K<64, GX_BF16, 4, U>)     \
+                                            : (a->bits == 16 ? K<64, GX_F16, 16, U> : K<64, GX_F16, 4, U>)))
+#define PC_PICK(K) (u == 4 ? PC_PICK_U(K, 4) : PC_PICK_U(K, 1))
 
-static int pc_launch(pc_fn f, const ThvmPagedArgs *a, uint32_t heads, const char *who, hipStream_t s, char *err,
+// Groups a wave: four, which find the row's place once, where that leaves the card
+// full of waves; else one, whose way is shorter.  kv_append's 12 groups a row of 48
+// heads of 128, one | four of them a wave, us: 1 row 2.8 | 4.0, 96 rows 3.7 | 5.0,
+// 384 rows 5.2 | 6.1, 768 rows (9216 groups) 8.0 | 8.0, 1536 rows 12.9 | 11.6.
+static uint32_t pc_groups(const ThvmPagedArgs *a, uint32_t heads) {
+  const uint32_t vpw = 64 / (a->hd / 8);
+  return (uint64_t)a->n * ((heads + vpw - 1) / vpw) >= 4 * PC_FILL ? 4 : 1;
+}
+
+static int pc_launch(pc_fn f, uint32_t u, const ThvmPagedArgs *a, uint32_t heads, const char *who, hipStream_t s, char *err,
                      int errlen) {
   const uint32_t vpw = 64 / (a->hd / 8);
-  const uint64_t waves = (uint64_t)a->n * (((heads + vpw - 1) / vpw + PC_U - 1) / PC_U);
+  const uint64_t waves = (uint64_t)a->n * (((heads + vpw - 1) / vpw + u - 1) / u);
   thvm_launch(true, true, f, dim3((uint32_t)((waves + 3) / 4)), dim3(PC_THREADS), 0, s, *a);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) { snprintf(err, errlen, "%s launch: %s", who, hipGetErrorString(e)); return -1; }
@@ -234,11 +248,13 @@ static int pc_launch(pc_fn f, const ThvmPagedArgs *a, uint32_t heads, const char
 extern "C" int thvm_k_kv_append(const ThvmPagedArgs *a, hipStream_t s, char *err, int errlen) {
   if (pg_check(a, PG_APPEND, err, errlen)) return -1;
   const int bf = a->dt == THVM_DT_BF16;
-  return pc_launch(PC_PICK(k_kv_append), a, a->H + 2 * a->Hkv, "kv_append", s, err, errlen);
+  const uint32_t u = pc_groups(a, a->H + 2 * a->Hkv);
+  return pc_launch(PC_PICK(k_kv_append), u, a, a->H + 2 * a->Hkv, "kv_append", s, err, errlen);
 }
 
 extern "C" int thvm_k_kv_read(const ThvmPagedArgs *a, hipStream_t s, char *err, int errlen) {
   if (pg_check(a, PG_READ, err, errlen)) return -1;
   const int bf = a->dt == THVM_DT_BF16;
-  return pc_launch(PC_PICK(k_kv_read), a, 2 * a->Hkv, "kv_read", s, err, errlen);
+  const uint32_t u = pc_groups(a, 2 * a->Hkv);
+  return pc_launch(PC_PICK(k_kv_read), u, a, 2 * a->Hkv, "kv_read", s, err, errlen);
 }
