@@ -124,15 +124,30 @@ __device__ __forceinline__ bool pg_unit(const ThvmPagedArgs &a, const PgPlan &p,
   float total = 0.0f, tiles = 0.0f;
   each([&](uint32_t, const PgSeq &, float t, float l) { total += wave_sum(t * l); tiles += wave_sum(t); });
   if (tiles == 0.0f) return false;
+  // steps in whole chunks of c, and the number with a shorter last one (l < 2^24)
+  auto chunks = [](float l, uint32_t c, float rc, float &full, float &per) {
+    uint32_t q = (uint32_t)(l * rc);
+    int32_t r = (int32_t)((uint32_t)l - q * c);            // q is off by one at most
+    if (r < 0) { q--; r += (int32_t)c; }
+    if (r >= (int32_t)c) { q++; r -= (int32_t)c; }
+    full = (float)q;
+    per = (float)(q + (r != 0));
+  };
   const float units = (float)p.units;
   const uint32_t c1 = max(p.cmin, (uint32_t)(total / units)), c2 = max(c1, (uint32_t)(total * 1.0001f / (units - tiles)) + 1);
   uint32_t c = c1;
+  float n, whole;
   for (int k = 1;; k++) {
-    if (k > 4) { c = c2; break; }
-    float n = 0.0f;
-    each([&](uint32_t, const PgSeq &, float t, float l) { n += wave_sum(t * (float)(((uint32_t)l + c - 1) / c)); });
-    if (n <= units) break;
-    c = c1 + (uint32_t)((uint64_t)(c2 - c1) * k / 4);
+    n = whole = 0.0f;
+    const float rc = __builtin_amdgcn_rcpf((float)c);
+    each([&](uint32_t, const PgSeq &, float t, float l) {
+      float full, per;
+      chunks(l, c, rc, full, per);
+      n += wave_sum(t * per);
+      whole += wave_sum(t * full);
+    });
+    if (n <= units || k > 4) break;
+    c = k == 4 ? c2 : c1 + (c2 - c1) * k / 4;
   }
   o.c = c;
   // the order of the blocks: whole chunks first, then the tiles' shorter last ones (all
@@ -140,21 +155,19 @@ __device__ __forceinline__ bool pg_unit(const ThvmPagedArgs &a, const PgPlan &p,
   uint32_t at = u;
   bool rest = false;
   if (!tiles_only) {
-    float whole = 0.0f, n = 0.0f;
-    each([&](uint32_t, const PgSeq &, float t, float l) {
-      whole += wave_sum(t * (float)((uint32_t)l / c));
-      n += wave_sum(t * (float)(((uint32_t)l + c - 1) / c));
-    });
     if ((float)u >= n) return false;
     rest = (float)u >= whole;
     at = rest ? u - (uint32_t)whole : u;
     if (whole == 0.0f) at = (uint32_t)n - 1 - u;
   }
+  const float rc = __builtin_amdgcn_rcpf((float)c);
   float before = 0.0f, kbefore = 0.0f;
   bool found = false;
   each([&](uint32_t s0, const PgSeq &q, float t, float l) {
     if (found) return;
-    const float per = (float)(((uint32_t)l + c - 1) / c), full = (float)((uint32_t)l / c), n = t * per;
+    float full, per;
+    chunks(l, c, rc, full, per);
+    const float n = t * per;
     const float key = tiles_only ? t : t * (rest ? per - full : full);
     const float sc = wave_scan(n), kc = wave_scan(key);
     const uint64_t hit = __builtin_amdgcn_ballot_w64(kbefore + kc > (float)at);
