@@ -23,7 +23,7 @@ __device__ __forceinline__ void pa_fold(const ThvmPagedArgs &a, const PgPlan &pl
   constexpr int LN = HD / 4, NG = 256 / LN, CB = NG / NP, BT = 8;   // lanes a chunk, groups, columns at once, loads ahead
   const uint32_t g = threadIdx.x / LN, x = threadIdx.x % LN, part = g % NP, G = a.H / a.Hkv;
   const uint64_t st = (uint64_t)CT * (HD + 4);
-  const float *const base = a.ws + ((uint64_t)kvh * pl.units + u.first) * st;
+  const float *const base = a.ws + ((uint64_t)kvh * pl.slots + u.first) * st;
   for (uint32_t c = c0 + g / NP; c < c1; c += CB) {        // (as many rounds for every thread)
     const uint32_t cc = u.tile * pl.ct + c;
     const bool live = (int32_t)(cc / G) < u.q.r1 - u.q.r0;
@@ -442,7 +442,7 @@ __global__ __launch_bounds__(PS_THREADS, 2) void k_paged_split(ThvmPagedArgs a, 
       const float inv = lt != 0.0f ? 1.0f / lt : 0.0f;
       *(uint32_t *)((uint16_t *)a.out + ((uint64_t)(u.q.r0 + cc / G) * a.H + kvh * G + cc % G) * HD + d) = P::pk(s0 * inv, s1 * inv);
     } else {
-      float *const rec = a.ws + ((uint64_t)kvh * pl.units + u.u) * CG * (HD + 4), *pp = rec + c * (HD + 4);
+      float *const rec = a.ws + ((uint64_t)kvh * pl.slots + u.u) * CG * (HD + 4), *pp = rec + c * (HD + 4);
       if (pl.fuse) {
         coh_st8(rec, (c * (HD + 4) + d) * 4, make_uint2(__float_as_uint(s0), __float_as_uint(s1)));
         if (d == 0) coh_st8(rec, (c * (HD + 4) + HD) * 4, make_uint2(__float_as_uint(M), __float_as_uint(lt)));
@@ -458,7 +458,7 @@ __global__ __launch_bounds__(PS_THREADS, 2) void k_paged_split(ThvmPagedArgs a, 
   vm_drain();
   __syncthreads();
   if (tid == 0) {
-    uint32_t *ctr = pa_arrived + (uint64_t)kvh * pl.units + u.first;
+    uint32_t *ctr = pa_arrived + (uint64_t)kvh * pl.slots + u.first;
     const uint32_t old = __hip_atomic_fetch_add(ctr, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     lastf = old == u.nchunk - 1 ? 1u : 0u;
     if (lastf) __hip_atomic_exchange(ctr, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -497,27 +497,34 @@ static PaRule pa_rule(const ThvmPagedArgs *a) {
   r.many = most > hi;
   r.few = !r.many || a->ragged;
   r.few_tiles = a->b * ((hi + 15) / 16);
-  r.fpl = PgPlan{0, hi, 16, fill > 2 * r.few_tiles ? fill : 2 * r.few_tiles, 4, 0};
+  r.fpl = PgPlan{0, hi, 16, fill > 2 * r.few_tiles ? fill : 2 * r.few_tiles, 4, 0, 0, 0};
+  // twice the units (see PgPlan) from 1.5 MB of cache a unit on: 32 ragged requests of
+  // up to 16000 rows 119 -> 108 us, 24 of 16000 each 280 -> 246; with a fifth of that
+  // twice the blocks lose (eight ragged requests of up to 8000 rows 29 -> 34 us)
+  const uint32_t step = 64 * 2 * (a->bits == 16 ? a->hd * 2 : a->hd / 2 + a->hd / 32);
+  r.fpl.cbig = (3u << 19) / step;
+  r.fpl.slots = r.fpl.units << ((uint64_t)r.few_tiles * a->maxpages * a->page / 64 >= (uint64_t)r.fpl.units * r.fpl.cbig);
   // about as many chunks as a tile can have, twice the mean where the units are shared
-  const uint64_t cap = ((uint64_t)a->maxpages * a->page + 64 * r.fpl.cmin - 1) / (64 * r.fpl.cmin), mean = 2 * r.fpl.units / r.few_tiles + 1;
-  const uint64_t chunks = cap < mean ? cap : mean < r.fpl.units ? mean : r.fpl.units;
-  r.fpl.fuse = chunks * r.cg <= 96 && (uint64_t)a->Hkv * r.fpl.units <= PA_COUNTERS &&
-               (uint64_t)r.fpl.units * r.cg * (a->hd + 4) * 4 < (1ull << 31);
+  const uint64_t cap = ((uint64_t)a->maxpages * a->page + 64 * r.fpl.cmin - 1) / (64 * r.fpl.cmin), mean = 2 * r.fpl.slots / r.few_tiles + 1;
+  const uint64_t chunks = cap < mean ? cap : mean < r.fpl.slots ? mean : r.fpl.slots;
+  r.fpl.fuse = chunks * r.cg <= 96 && (uint64_t)a->Hkv * r.fpl.slots <= PA_COUNTERS &&
+               (uint64_t)r.fpl.slots * r.cg * (a->hd + 4) * 4 < (1ull << 31);
   const uint32_t whole = (uint32_t)((uint64_t)a->n * G / PP_COLS);
   r.many_tiles = whole + a->b;
   r.split = (uint64_t)whole * a->Hkv < 512;
-  r.mpl = PgPlan{r.few ? hi : 0, 0xffffffffu, PP_COLS, r.many_tiles + 1, 1u << 25, 0};
+  r.mpl = PgPlan{r.few ? hi : 0, 0xffffffffu, PP_COLS, r.many_tiles + 1, 1u << 25, 0, 0, 0};
   if (r.split) {
     r.mpl.units = fill > 2 * r.many_tiles ? fill : 2 * r.many_tiles;
     r.mpl.cmin = 4;
   }
+  r.mpl.slots = r.mpl.units;
   return r;
 }
 
 extern "C" uint64_t thvm_k_attn_paged_ws(const ThvmPagedArgs *a) {
   const PaRule r = pa_rule(a);
-  const uint64_t rec = (uint64_t)a->Hkv * (a->hd + 4) * 4, f = r.few ? rec * r.fpl.units * r.cg : 0,
-                 m = r.many && r.split ? rec * r.mpl.units * PP_COLS : 0;
+  const uint64_t rec = (uint64_t)a->Hkv * (a->hd + 4) * 4, f = r.few ? rec * r.fpl.slots * r.cg : 0,
+                 m = r.many && r.split ? rec * r.mpl.slots * PP_COLS : 0;
   return f > m ? f : m > 16 ? m : 16;
 }
 
@@ -542,12 +549,12 @@ extern "C" int thvm_k_attn_paged(const ThvmPagedArgs *a, hipStream_t s, char *er
                                    : (bf ? pa_pick<64, GX_BF16>(a, r.cg) : pa_pick<64, GX_F16>(a, r.cg));
   if (r.few) {
     const bool last = !r.many;
-    thvm_launch(true, last && r.fpl.fuse, k.split, dim3(a->Hkv * r.fpl.units), dim3(PS_THREADS), 0, s, *a, r.fpl);
+    thvm_launch(true, last && r.fpl.fuse, k.split, dim3(a->Hkv * r.fpl.slots), dim3(PS_THREADS), 0, s, *a, r.fpl);
     if (!r.fpl.fuse)
       thvm_launch(false, last, k.merge, dim3(a->Hkv * r.cg * r.few_tiles), dim3(256), 0, s, *a, r.fpl);
   }
   if (r.many) {
-    thvm_launch(!r.few, !r.split, pp_tile_pick(a), dim3(a->Hkv * r.mpl.units), dim3(PP_THREADS), 0, s, *a, r.mpl);
+    thvm_launch(!r.few, !r.split, pp_tile_pick(a), dim3(a->Hkv * r.mpl.slots), dim3(PP_THREADS), 0, s, *a, r.mpl);
     if (r.split)
       thvm_launch(false, true, k.tmerge, dim3(a->Hkv * (PP_COLS / PA_MERGE) * r.many_tiles), dim3(256), 0, s, *a, r.mpl);
   }

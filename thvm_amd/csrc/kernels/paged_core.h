@@ -79,9 +79,12 @@ template <bool V> struct pg_const { static constexpr bool value = V; };
 // try always does (a tile adds one chunk at most to its share); the host launches
 // units >= 2 x tiles, so c never passes the mean length of the tiles: long
 // sequences are split, short ones are not, and the blocks are of one size but for
-// the last chunk of each tile.  Those come after the whole ones.  `fuse`: the last
-// block of a tile adds its chunks.
-struct PgPlan { uint32_t lo, hi, ct, units, cmin, fuse; };
+// the last chunk of each tile.  Those come after the whole ones.  Where that fills
+// less than 0.8 of units x c (short tiles, lengths that c divides badly), `slots` is
+// twice `units` and c at least cbig, it is done again with twice the units: a second
+// round of blocks costs some 7 us and evens out.  `fuse`: the last block of a tile
+// adds its chunks.
+struct PgPlan { uint32_t lo, hi, ct, units, cmin, fuse, slots, cbig; };
 struct PgUnit { PgSeq q; uint32_t s, tile, chunk, nchunk, c, first, u; };
 
 __device__ __forceinline__ float wave_scan(float v) {           // inclusive, lane order
@@ -133,21 +136,24 @@ __device__ __forceinline__ bool pg_unit(const ThvmPagedArgs &a, const PgPlan &p,
     full = (float)q;
     per = (float)(q + (r != 0));
   };
-  const float units = (float)p.units;
-  const uint32_t c1 = max(p.cmin, (uint32_t)(total / units)), c2 = max(c1, (uint32_t)(total * 1.0001f / (units - tiles)) + 1);
-  uint32_t c = c1;
+  uint32_t c;
   float n, whole;
-  for (int k = 1;; k++) {
-    n = whole = 0.0f;
-    const float rc = __builtin_amdgcn_rcpf((float)c);
-    each([&](uint32_t, const PgSeq &, float t, float l) {
-      float full, per;
-      chunks(l, c, rc, full, per);
-      n += wave_sum(t * per);
-      whole += wave_sum(t * full);
-    });
-    if (n <= units || k > 4) break;
-    c = k == 4 ? c2 : c1 + (c2 - c1) * k / 4;
+  for (float units = (float)p.units;; units *= 2.0f) {
+    const uint32_t c1 = max(p.cmin, (uint32_t)(total / units)), c2 = max(c1, (uint32_t)(total * 1.0001f / (units - tiles)) + 1);
+    c = c1;
+    for (int k = 1;; k++) {
+      n = whole = 0.0f;
+      const float rc = __builtin_amdgcn_rcpf((float)c);
+      each([&](uint32_t, const PgSeq &, float t, float l) {
+        float full, per;
+        chunks(l, c, rc, full, per);
+        n += wave_sum(t * per);
+        whole += wave_sum(t * full);
+      });
+      if (n <= units || k > 4) break;
+      c = k == 4 ? c2 : c1 + (c2 - c1) * k / 4;
+    }
+    if (units >= (float)p.slots || c < p.cbig || total >= 0.8f * units * (float)c) break;
   }
   o.c = c;
   // the order of the blocks: whole chunks first, then the tiles' shorter last ones (all

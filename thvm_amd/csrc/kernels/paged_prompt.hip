@@ -385,7 +385,7 @@ __global__ __launch_bounds__(PP_THREADS, 2) void k_paged_tile(ThvmPagedArgs a, P
         *(uint2 *)(o + 32 * d + 8 * q) = make_uint2(P::pk(acc[d][4 * q] * inv, acc[d][4 * q + 1] * inv),
                                                     P::pk(acc[d][4 * q + 2] * inv, acc[d][4 * q + 3] * inv));
   } else {
-    float *pp = a.ws + (((uint64_t)kvh * pl.units + u.u) * PP_COLS + 32 * wv + n) * (HD + 4);
+    float *pp = a.ws + (((uint64_t)kvh * pl.slots + u.u) * PP_COLS + 32 * wv + n) * (HD + 4);
 #pragma unroll
     for (int d = 0; d < DB; d++)
 #pragma unroll
