@@ -496,7 +496,7 @@ static PaRule pa_rule(const ThvmPagedArgs *a) {
   const uint32_t hi = most <= 16 || r.cg > G ? r.cg : G;
   r.many = most > hi;
   r.few = !r.many || a->ragged;
-  r.few_tiles = a->b * ((hi + 15) / 16);
+  r.few_tiles = (a->b < a->n ? a->b : a->n) * ((hi + 15) / 16);   // (of sequences with a row)
   r.fpl = PgPlan{0, hi, 16, fill > 2 * r.few_tiles ? fill : 2 * r.few_tiles, 4, 0, 0, 0};
   // twice the units (see PgPlan) from 1.5 MB of cache a unit on: 32 ragged requests of
   // up to 16000 rows 119 -> 108 us, 24 of 16000 each 280 -> 246; with a fifth of that
@@ -510,7 +510,7 @@ static PaRule pa_rule(const ThvmPagedArgs *a) {
   r.fpl.fuse = chunks * r.cg <= 96 && (uint64_t)a->Hkv * r.fpl.slots <= PA_COUNTERS &&
                (uint64_t)r.fpl.slots * r.cg * (a->hd + 4) * 4 < (1ull << 31);
   const uint32_t whole = (uint32_t)((uint64_t)a->n * G / PP_COLS);
-  r.many_tiles = whole + a->b;
+  r.many_tiles = whole + (a->b < a->n ? a->b : a->n);
   r.split = (uint64_t)whole * a->Hkv < 512;
   r.mpl = PgPlan{r.few ? hi : 0, 0xffffffffu, PP_COLS, r.many_tiles + 1, 1u << 25, 0, 0, 0};
   if (r.split) {

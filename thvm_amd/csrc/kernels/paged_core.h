@@ -155,6 +155,7 @@ __device__ __forceinline__ bool pg_unit(const ThvmPagedArgs &a, const PgPlan &p,
     }
     if (units >= (float)p.slots || c < p.cbig || total >= 0.8f * units * (float)c) break;
   }
+  if (n > (float)p.slots) return false;                    // row offsets that overlap: nothing is done
   o.c = c;
   // the order of the blocks: whole chunks first, then the tiles' shorter last ones (all
   // of a tile where none is split: backwards, as a prompt's last tiles see most)
