@@ -122,7 +122,7 @@ template <> struct PsRegs<128, 4> { uint4 k[4]; uint32_t ks[4]; uint32_t v[4][4]
 template <> struct PsRegs<64, 4> { uint2 k[4]; uint32_t ks[4]; uint32_t v[4][4]; uint2 vs[4]; };
 
 template <int HD, int XT, int BITS, int CG>
-__global__ __launch_bounds__(PS_THREADS, 2) void k_paged_split(ThvmPagedArgs a, PgPlan pl) {
+__global__ __launch_bounds__(PS_THREADS, HD == 64 && BITS == 4 ? (CG == 8 ? 3 : 4) : 2) void k_paged_split(ThvmPagedArgs a, PgPlan pl) {
   typedef PgT<XT> P;
   constexpr int EC = HD / 16, KS = HD / 32, NG = 16 / CG, NS = 4 / NG, RB = BITS == 16 ? HD * 2 : HD / 2;
   constexpr uint32_t EXP = XT == GX_BF16 ? 0x7f80u : 0x7c00u;
@@ -497,12 +497,16 @@ static PaRule pa_rule(const ThvmPagedArgs *a) {
   r.many = most > hi;
   r.few = !r.many || a->ragged;
   r.few_tiles = (a->b < a->n ? a->b : a->n) * ((hi + 15) / 16);   // (of sequences with a row)
-  r.fpl = PgPlan{0, hi, 16, fill > 2 * r.few_tiles ? fill : 2 * r.few_tiles, 4, 0, 0, 0};
+  r.fpl = PgPlan{0, hi, 16, fill > 2 * r.few_tiles ? fill : 2 * r.few_tiles, 4, 0, 0, 0, 0.8f};
   // twice the units (see PgPlan) from 1.5 MB of cache a unit on: 32 ragged requests of
   // up to 16000 rows 119 -> 108 us, 24 of 16000 each 280 -> 246; with a fifth of that
   // twice the blocks lose (eight ragged requests of up to 8000 rows 29 -> 34 us)
   const uint32_t step = 64 * 2 * (a->bits == 16 ? a->hd * 2 : a->hd / 2 + a->hd / 32);
   r.fpl.cbig = (3u << 19) / step;
+  // heads of 64 in 4 bits: registers for four blocks a CU, so twice the units from 40
+  // steps on (16 requests of 16000 rows 48.5 -> 42.9 us, 25 heads x 4 of 100000 191 ->
+  // 166; below, four of 16000 lose: 19.5 -> 20.9)
+  if (a->hd == 64 && a->bits == 4) { r.fpl.cbig = 40; r.fpl.even = 2.0f; }
   r.fpl.slots = r.fpl.units << ((uint64_t)r.few_tiles * a->maxpages * a->page / 64 >= (uint64_t)r.fpl.units * r.fpl.cbig);
   // about as many chunks as a tile can have, twice the mean where the units are shared
   const uint64_t cap = ((uint64_t)a->maxpages * a->page + 64 * r.fpl.cmin - 1) / (64 * r.fpl.cmin), mean = 2 * r.fpl.slots / r.few_tiles + 1;
@@ -512,7 +516,7 @@ static PaRule pa_rule(const ThvmPagedArgs *a) {
   const uint32_t whole = (uint32_t)((uint64_t)a->n * G / PP_COLS);
   r.many_tiles = whole + (a->b < a->n ? a->b : a->n);
   r.split = (uint64_t)whole * a->Hkv < 512;
-  r.mpl = PgPlan{r.few ? hi : 0, 0xffffffffu, PP_COLS, r.many_tiles + 1, 1u << 25, 0, 0, 0};
+  r.mpl = PgPlan{r.few ? hi : 0, 0xffffffffu, PP_COLS, r.many_tiles + 1, 1u << 25, 0, 0, 0, 0.0f};
   if (r.split) {
     r.mpl.units = fill > 2 * r.many_tiles ? fill : 2 * r.many_tiles;
     r.mpl.cmin = 4;

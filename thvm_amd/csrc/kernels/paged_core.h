@@ -80,11 +80,11 @@ template <bool V> struct pg_const { static constexpr bool value = V; };
 // units >= 2 x tiles, so c never passes the mean length of the tiles: long
 // sequences are split, short ones are not, and the blocks are of one size but for
 // the last chunk of each tile.  Those come after the whole ones.  Where that fills
-// less than 0.8 of units x c (short tiles, lengths that c divides badly), `slots` is
+// less than `even` of units x c (short tiles, lengths that c divides badly), `slots` is
 // twice `units` and c at least cbig, it is done again with twice the units: a second
 // round of blocks costs some 7 us and evens out.  `fuse`: the last block of a tile
 // adds its chunks.
-struct PgPlan { uint32_t lo, hi, ct, units, cmin, fuse, slots, cbig; };
+struct PgPlan { uint32_t lo, hi, ct, units, cmin, fuse, slots, cbig; float even; };
 struct PgUnit { PgSeq q; uint32_t s, tile, chunk, nchunk, c, first, u; };
 
 __device__ __forceinline__ float wave_scan(float v) {           // inclusive, lane order
@@ -153,7 +153,7 @@ __device__ __forceinline__ bool pg_unit(const ThvmPagedArgs &a, const PgPlan &p,
       if (n <= units || k > 4) break;
       c = k == 4 ? c2 : c1 + (c2 - c1) * k / 4;
     }
-    if (units >= (float)p.slots || c < p.cbig || total >= 0.8f * units * (float)c) break;
+    if (units >= (float)p.slots || c < p.cbig || total >= p.even * units * (float)c) break;
   }
   if (n > (float)p.slots) return false;                    // row offsets that overlap: nothing is done
   o.c = c;
