@@ -81,7 +81,15 @@ __global__ __launch_bounds__(PC_THREADS) void k_kv_append(ThvmPagedArgs a) {
       c[k] = cc.x; c[k + 1] = cc.y; c[k + 2] = cc.z; c[k + 3] = cc.w;
       sn[k] = ss.x; sn[k + 1] = ss.y; sn[k + 2] = ss.z; sn[k + 3] = ss.w;
     }
+    if (a.rope == 2 && d0 < HD / 2) {                  // x c - o s there, x c + o s in the upper half
+#pragma unroll
+      for (int k = 0; k < 8; k++) sn[k] = -sn[k];
+    }
   }
+  // (wave-uniform: a group of v heads alone is copied)
+  bool turned[U];
+#pragma unroll
+  for (int u = 0; u < U; u++) turned[u] = (g0 + u) * VPW < a.H + a.Hkv;
   float inv[U];
   if (a.norm) {
     // each lane has its head's sums of all groups: it takes one of them through the
@@ -89,6 +97,7 @@ __global__ __launch_bounds__(PC_THREADS) void k_kv_append(ThvmPagedArgs a) {
     double one = 0.0;
 #pragma unroll
     for (int u = 0; u < U; u++) {
+      if (!turned[u]) break;
       const uint32_t w[4] = {x[u].x, x[u].y, x[u].z, x[u].w};
       double ss = 0.0;
 #pragma unroll
@@ -126,14 +135,14 @@ __global__ __launch_bounds__(PC_THREADS) void k_kv_append(ThvmPagedArgs a) {
     float v[8];
 #pragma unroll
     for (int i = 0; i < 4; i++) { v[2 * i] = P::lo(xw[i]); v[2 * i + 1] = P::hi(xw[i]); }
-    if (a.norm && !isv) {
+    if (a.norm && turned[u] && !isv) {
       const float *g = (isq ? a.gq : a.gk) + d0;
       const float4 ga = *(const float4 *)g, gb = *(const float4 *)(g + 4);
       const float gg[8] = {ga.x, ga.y, ga.z, ga.w, gb.x, gb.y, gb.z, gb.w};
 #pragma unroll
       for (int i = 0; i < 8; i++) v[i] = (v[i] * inv[u]) * gg[i];
     }
-    if (a.rope && placed) {
+    if (a.rope && placed && turned[u]) {
       if (a.rope == 1) {
 #pragma unroll
         for (int k = 0; k < 4; k++) {
@@ -145,7 +154,7 @@ __global__ __launch_bounds__(PC_THREADS) void k_kv_append(ThvmPagedArgs a) {
 #pragma unroll
         for (int k = 0; k < 8; k++) {                  // the partner is half a head away
           const float o = LPV == 16 ? dpp_f<0x128>(v[k]) : __shfl_xor(v[k], 4);
-          const float y = d0 < HD / 2 ? v[k] * c[k] - o * sn[k] : v[k] * c[k] + o * sn[k];
+          const float y = v[k] * c[k] + o * sn[k];
           v[k] = isv ? v[k] : y;
         }
       }
