@@ -301,7 +301,9 @@ int thvm_k_moe_down(const ThvmMoeArgs *a, hipStream_t s, char *err, int errlen);
  * H, Hkv, hd, max_seq, qdt, cdt, odt, scale and T. */
 int thvm_k_attn_prompt(const ThvmAttnArgs *a, hipStream_t s, char *err, int errlen);
 
-/* A paged cache and the calls on it.  n rows (new positions) of b sequences:
+/* A paged cache and the calls on it.  (attn_paged counts a tile's finished blocks in
+ * a device array of its own, zero between launches: calls on one GPU run one after
+ * another, as everything on the library's stream does.)  n rows (new positions) of b sequences:
  * sequence s has the rows [rows[s], rows[s+1]) of the call (rows NULL: n / b
  * each), the last ones of its len[s] cache rows, so row i of them is position
  * len[s] - count + i.  A pool holds npages pages of [Hkv][page] rows of one

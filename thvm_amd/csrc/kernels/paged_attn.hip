@@ -110,7 +110,11 @@ static __device__ uint32_t pa_arrived[PA_COUNTERS];
 // the q operand is ordered to match.  p enters the product as a pair of 16-bit terms
 // (hi and what it leaves: 16 bits of p in bf16, 22 in fp16), which costs nothing where
 // the cache's bytes are the bound; its sum, like all else, is f32.
-// Bound by the cache's bytes.
+// Bound by the cache's bytes: over 16 bits 16 requests of 30000 rows (8 kv heads of
+// 128, 4 query heads each) run at 6.4 TB/s, 32 ragged ones of up to 16000 rows at 5.5;
+// over 4 bits 16 of 100000 rows at 5.3 TB/s, where the codec's instructions and the
+// loads share a SIMD's two waves.  Short contexts: some 7 us of dependent steps (plan,
+// page ids, rows, hand-off), 11 us for one request of 2049 rows.
 #define PS_WAVES 4
 #define PS_THREADS (PS_WAVES * 64)
 

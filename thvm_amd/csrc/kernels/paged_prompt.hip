@@ -21,7 +21,10 @@
 // and p has room: up to 2^6 in bf16, 2^14 of fp16's 2^16 with p scaled by 2^8,
 // which keeps small p off fp16's subnormals); p is rounded once, to the 16-bit type
 // of the values it multiplies, and its sum, in f32, is that of the rounded ones.
-// Bound by the matrix and exponential units.
+// Bound by the matrix and exponential units: five ragged prompts of up to 3001 rows (8
+// kv heads of 128, 4 query heads each) in 250 us, 820 TFLOP/s.  The products alone take
+// 183 us of it (1136 TFLOP/s), loads and exponents what does not overlap.  Blocks of 8
+// waves lose (266 us), so do deeper prefetch and wave priorities (no change).
 #include "paged_core.h"
 
 #define PP_STEP 64
