@@ -58,6 +58,48 @@ def test_attn_paged_wide_batches(hip, bits, H, Hkv, hd, seqs):
     check_attn(P, q, kp, vp, attn(hip, P, q, kp, vp, scale), scale)
 
 
+@pytest.mark.parametrize("dt,bits,H,Hkv,hd,page", [(DT_BF16, 16, 4, 1, 64, 16), (DT_F16, 4, 4, 2, 128, 32)])
+@pytest.mark.parametrize("b", [66, 257, 700, 4096])
+def test_paged_many_requests(hip, dt, bits, H, Hkv, hd, page, b):
+    """Hundreds of requests in one ragged call, tokens beside prompts and empty ones:
+    appended, read back and attended."""
+    say(f"case: paged b={b} dt={dt} bits={bits} H={H} Hkv={Hkv} hd={hd}")
+    n = [0 if i % 7 == 3 else 40 if i % 97 == 65 else 1 + (i % 5 == 0) for i in range(b)]
+    P, q, kp, vp, scale = case([(r, r + 29 * i % 300 + 700 * (i % 59 == 1)) for i, r in enumerate(n)], dt, bits, H, Hkv,
+                               hd, page, extra=2)
+    x = P.make_x()
+    got = append(hip, P, x, kp, vp)
+    check_append(P, x, kp, vp, got)
+    check_attn(P, q, got[1], got[2], attn(hip, P, q, got[1], got[2], scale), scale)
+    check_attn(P, q, got[1], got[2], attn(hip, P, q, got[1], got[2], scale, t=40), scale)
+    k, v = (kept(hip, P.n * Hkv * hd * 2) for _ in range(2))
+    hip.builtin("kv_read", [k, v, up(hip, got[1]), up(hip, got[2])] + index_args(hip, P), outs=(0, 1), **P.spec())
+    kheld = P.held(got[1])
+    k = O.decode(k.read(np.uint16).reshape(P.n, Hkv, hd), dt).astype(np.float64)
+    for row, s, pos in P.each_row():
+        pg, slot = P.where(s, pos)
+        assert np.array_equal(k[row], kheld[pg, :, slot]), (row, s, pos)
+
+
+def test_attn_paged_garbage_of_many_requests(hip):
+    """Offsets, lengths and pages of hundreds of requests full of garbage: the calls
+    end inside their buffers, and a good one after them is right."""
+    say("case: garbage of many requests")
+    rng = np.random.default_rng(8)
+    P, q, kp, vp, scale = case([(1 + i % 3, 20 + 7 * i % 400) for i in range(300)], DT_BF16, 16, 4, 1, 64, 16)
+    good = attn(hip, P, q, kp, vp, scale)
+    rows, ln, table = P.rows.copy(), P.len.copy(), P.table.copy()
+    for i in range(5):
+        P.rows = rng.integers(-2 ** 31, 2 ** 31, rows.shape).astype(np.int32) if i % 2 else rng.permutation(rows)
+        P.len = rng.integers(-2 ** 31, 2 ** 31, ln.shape).astype(np.int32) if i % 3 else ln
+        P.table = rng.integers(-2 ** 31, 2 ** 31, table.shape).astype(np.int32) if i % 4 > 1 else table
+        attn(hip, P, q, kp, vp, scale)
+        append(hip, P, P.make_x(), kp, vp)
+    P.rows, P.len, P.table = rows, ln, table
+    assert np.array_equal(attn(hip, P, q, kp, vp, scale), good)
+    check_attn(P, q, kp, vp, good, scale)
+
+
 @pytest.mark.parametrize("bits", [16, 4])
 @pytest.mark.parametrize("b,ctx", [(24, 16000), (9, 70000)])
 def test_attn_paged_twice_the_chunks(hip, bits, b, ctx):
@@ -103,6 +145,41 @@ def test_attn_paged_offsets_that_overlap(hip):
         again = attn(hip, P, q, kp, vp, scale)
         assert np.array_equal(again, first)
         check_attn(P, q, kp, vp, again, scale)
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("page", [16, 128])
+def test_paged_far_pages_of_prompts(hip, bits, page):
+    """A prompt's rows in pages past 4 GiB of their pool: appended, read and attended."""
+    say(f"case: a prompt's pages past 4 GiB, bits={bits} page={page}")
+    P, q, kp, vp, scale = case([(40, 90), (17, 17)], DT_BF16, bits, 8, 8, 128, page)
+    x = P.make_x()
+    want = append(hip, P, x, kp, vp)
+    ref = attn(hip, P, q, want[1], want[2], scale)
+    check_attn(P, q, want[1], want[2], ref, scale)
+    blk = 8 * page * P.rb
+    far, near_, n0 = (5 << 30) // blk, P.table.copy(), P.npages
+    bufs = []
+    for pool in (kp, vp):
+        bufs.append(hip.Buffer((far + n0) * blk))
+        bufs[-1].write(pool, far * blk)
+    P.table, P.npages = np.where(near_ >= 0, near_ + far, near_).astype(np.int32), far + n0
+    ix = index_args(hip, P)
+    qo, out, k, v = (kept(hip, P.n * 8 * 128 * 2) for _ in range(4))
+    kw = P.spec(h=8, scale=float(scale))
+    hip.builtin("kv_append", [qo] + bufs + [up(hip, x)] + ix, outs=(0, 1, 2), **P.spec(h=8))
+    hip.builtin("attn_paged", [out, up(hip, q)] + bufs + ix + [kept(hip, hip.attn_paged_ws(**kw))], **kw)
+    hip.builtin("kv_read", [k, v] + bufs + ix, outs=(0, 1), **P.spec())
+    assert np.array_equal(qo.read(np.uint16).reshape(want[0].shape), want[0])
+    assert np.array_equal(out.read(np.uint16).reshape(ref.shape), ref)
+    P.table, P.npages = near_, n0
+    for got, pool in ((k, want[1]), (v, want[2])):
+        held, got = P.held(pool), O.decode(got.read(np.uint16).reshape(P.n, 8, 128), DT_BF16).astype(np.float64)
+        for row, s, pos in P.each_row():
+            pg, slot = P.where(s, pos)
+            assert np.array_equal(got[row], held[pg, :, slot]), row
+    for b in bufs:
+        b.free()
 
 
 def test_attn_paged_graphs_share_a_workspace(hip):

@@ -487,6 +487,72 @@ __global__ __launch_bounds__(256) void k_paged_merge(ThvmPagedArgs a, PgPlan pl)
   pa_fold<HD, XT, CT, NP, false>(a, pl, u, blockIdx.x / (CT / CB) % a.Hkv, ls, lm, ll, c0, c0 + CB);
 }
 
+// k_paged_plan: the plans of a batch of more than 64 sequences, one block each; a
+// thread has up to four sequences in a row.  With it 1024 requests of 100 rows take 149
+// us, 512 of 1000 rows 403; with the plan in every wave, 64 sequences at a time, 518
+// and 496 (65 requests of 100 rows: 17 us there, a launch more here).
+#define PL_THREADS 1024
+__global__ __launch_bounds__(PL_THREADS) void k_paged_plan(ThvmPagedArgs a, PgPlan p0, PgPlan p1) {
+  const PgPlan p = blockIdx.x ? p1 : p0;
+  __shared__ float part[PL_THREADS / 64][2];
+  const uint32_t tid = threadIdx.x, wv = tid >> 6, s0 = 4 * tid, bb = (a.b + 3) & ~3u;
+  uint32_t *const pre = (uint32_t *)p.pre;
+  // (sums of two values over the block, and with scan what the threads before have)
+  auto sum2 = [&](float &x, float &y, bool scan) {
+    const float xs = wave_scan(x), ys = wave_scan(y);
+    __syncthreads();
+    if ((tid & 63) == 63) { part[wv][0] = xs; part[wv][1] = ys; }
+    __syncthreads();
+    float X = 0.0f, Y = 0.0f;
+    for (uint32_t w = 0; w < (scan ? wv : blockDim.x / 64); w++) { X += part[w][0]; Y += part[w][1]; }
+    x = scan ? X + xs - x : X;
+    y = scan ? Y + ys - y : Y;
+  };
+  float t[4], l[4], total = 0.0f, tiles = 0.0f, n, whole;
+#pragma unroll
+  for (int k = 0; k < 4; k++) {
+    PgSeq q;
+    t[k] = 0.0f;
+    l[k] = 1.0f;
+    if (s0 + k < a.b) pg_count(a, p, s0 + k, q, t[k], l[k]);
+    total += t[k] * l[k];
+    tiles += t[k];
+  }
+  sum2(total, tiles, false);
+  float full, per, tb = 0.0f, z = 0.0f, nb = 0.0f, wb = 0.0f;
+  const uint32_t c = pg_choose(p, total, tiles, [&](uint32_t c, float &sn, float &sw) {
+    sn = sw = 0.0f;
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+      pg_chunks(l[k], c, full, per);
+      sn += t[k] * per;
+      sw += t[k] * full;
+    }
+    sum2(sn, sw, false);
+  }, n, whole);
+#pragma unroll
+  for (int k = 0; k < 4; k++) {
+    pg_chunks(l[k], c, full, per);
+    tb += t[k];
+    nb += t[k] * per;
+    wb += t[k] * full;
+  }
+  sum2(tb, z, true);
+  sum2(nb, wb, true);
+  if (tid == 0) *(uint4 *)pre = make_uint4(c, (uint32_t)n, (uint32_t)whole, (uint32_t)tiles);
+#pragma unroll
+  for (int k = 0; k < 4; k++)
+    if (s0 + k < a.b) {
+      pre[4 + s0 + k] = (uint32_t)tb;
+      pre[4 + bb + s0 + k] = (uint32_t)nb;
+      pre[4 + 2 * bb + s0 + k] = (uint32_t)wb;
+      pg_chunks(l[k], c, full, per);
+      tb += t[k];
+      nb += t[k] * per;
+      wb += t[k] * full;
+    }
+}
+
 // ---- which kernels a call takes ------------------------------------------------
 // few: sequences of up to few.hi columns, cg of the MFMA's 16 columns used; many:
 // the others, chunks of them (split) where their tiles do not fill the chip.
@@ -501,7 +567,7 @@ static PaRule pa_rule(const ThvmPagedArgs *a) {
   r.many = most > hi;
   r.few = !r.many || a->ragged;
   r.few_tiles = (a->b < a->n ? a->b : a->n) * ((hi + 15) / 16);   // (of sequences with a row)
-  r.fpl = PgPlan{0, hi, 16, fill > 2 * r.few_tiles ? fill : 2 * r.few_tiles, 4, 0, 0, 0, 0.8f};
+  r.fpl = PgPlan{0, hi, 16, fill > 2 * r.few_tiles ? fill : 2 * r.few_tiles, 4, 0, 0, 0, 0.8f, nullptr};
   // twice the units (see PgPlan) from 1.5 MB of cache a unit on: 32 ragged requests of
   // up to 16000 rows 119 -> 108 us, 24 of 16000 each 280 -> 246; with a fifth of that
   // twice the blocks lose (eight ragged requests of up to 8000 rows 29 -> 34 us)
@@ -520,7 +586,7 @@ static PaRule pa_rule(const ThvmPagedArgs *a) {
   const uint32_t whole = (uint32_t)((uint64_t)a->n * G / PP_COLS);
   r.many_tiles = whole + (a->b < a->n ? a->b : a->n);
   r.split = (uint64_t)whole * a->Hkv < 512;
-  r.mpl = PgPlan{r.few ? hi : 0, 0xffffffffu, PP_COLS, r.many_tiles + 1, 1u << 25, 0, 0, 0, 0.0f};
+  r.mpl = PgPlan{r.few ? hi : 0, 0xffffffffu, PP_COLS, r.many_tiles + 1, 1u << 25, 0, 0, 0, 0.0f, nullptr};
   if (r.split) {
     r.mpl.units = fill > 2 * r.many_tiles ? fill : 2 * r.many_tiles;
     r.mpl.cmin = 4;
@@ -529,11 +595,14 @@ static PaRule pa_rule(const ThvmPagedArgs *a) {
   return r;
 }
 
+// words of the plans at the workspace's start: one for each half of the rule
+static uint64_t pa_pre_words(const ThvmPagedArgs *a) { return a->b > 64 ? 2 * PG_PRE_WORDS((uint64_t)a->b) : 0; }
+
 extern "C" uint64_t thvm_k_attn_paged_ws(const ThvmPagedArgs *a) {
   const PaRule r = pa_rule(a);
   const uint64_t rec = (uint64_t)a->Hkv * (a->hd + 4) * 4, f = r.few ? rec * r.fpl.slots * r.cg : 0,
                  m = r.many && r.split ? rec * r.mpl.slots * PP_COLS : 0;
-  return f > m ? f : m > 16 ? m : 16;
+  return (f > m ? f : m > 16 ? m : 16) + pa_pre_words(a) * 4;
 }
 
 template <int HD, int XT, int BITS>
@@ -549,20 +618,29 @@ static PaKernels pa_pick(const ThvmPagedArgs *a, uint32_t cg) {
                    k_paged_merge<HD, XT, PP_COLS, 1, PA_MERGE>};
 }
 
-extern "C" int thvm_k_attn_paged(const ThvmPagedArgs *a, hipStream_t s, char *err, int errlen) {
-  if (pg_check(a, PG_ATTN, err, errlen)) return -1;
-  const PaRule r = pa_rule(a);
+extern "C" int thvm_k_attn_paged(const ThvmPagedArgs *call, hipStream_t s, char *err, int errlen) {
+  if (pg_check(call, PG_ATTN, err, errlen)) return -1;
+  ThvmPagedArgs args = *call, *const a = &args;
+  PaRule r = pa_rule(a);
   const int bf = a->dt == THVM_DT_BF16;
   const PaKernels k = a->hd == 128 ? (bf ? pa_pick<128, GX_BF16>(a, r.cg) : pa_pick<128, GX_F16>(a, r.cg))
                                    : (bf ? pa_pick<64, GX_BF16>(a, r.cg) : pa_pick<64, GX_F16>(a, r.cg));
+  const bool plan = a->b > 64;
+  if (plan) {
+    r.fpl.pre = (const uint32_t *)a->ws;
+    r.mpl.pre = r.fpl.pre + PG_PRE_WORDS(a->b);
+    a->ws += pa_pre_words(a);
+    thvm_launch(true, false, k_paged_plan, dim3(r.few && r.many ? 2 : 1), dim3((a->b + 255) / 256 * 64), 0, s, *a,
+                r.few ? r.fpl : r.mpl, r.mpl);
+  }
   if (r.few) {
     const bool last = !r.many;
-    thvm_launch(true, last && r.fpl.fuse, k.split, dim3(a->Hkv * r.fpl.slots), dim3(PS_THREADS), 0, s, *a, r.fpl);
+    thvm_launch(!plan, last && r.fpl.fuse, k.split, dim3(a->Hkv * r.fpl.slots), dim3(PS_THREADS), 0, s, *a, r.fpl);
     if (!r.fpl.fuse)
       thvm_launch(false, last, k.merge, dim3(a->Hkv * r.cg * r.few_tiles), dim3(256), 0, s, *a, r.fpl);
   }
   if (r.many) {
-    thvm_launch(!r.few, !r.split, pp_tile_pick(a), dim3(a->Hkv * r.mpl.slots), dim3(PP_THREADS), 0, s, *a, r.mpl);
+    thvm_launch(!plan && !r.few, !r.split, pp_tile_pick(a), dim3(a->Hkv * r.mpl.slots), dim3(PP_THREADS), 0, s, *a, r.mpl);
     if (r.split)
       thvm_launch(false, true, k.tmerge, dim3(a->Hkv * (PP_COLS / PA_MERGE) * r.many_tiles), dim3(256), 0, s, *a, r.mpl);
   }

@@ -28,15 +28,19 @@ template <> struct PgT<GX_F16> {
 };
 
 // the sequence of row r, wave-uniform r: the one whose rows end first behind r
-// (a ballot over 64 ends at a time), or b for a row of none
+// (a ballot over 64 ends, beyond 64 sequences over every 64th before), or b or more
+// for a row of none
 __device__ __forceinline__ uint32_t pg_seq_of(const ThvmPagedArgs &a, uint32_t r) {
   if (!a.rows) return r / (a.n / a.b);
-  for (uint32_t s0 = 0; s0 < a.b; s0 += 64) {
-    const uint32_t s = s0 + lane_id();
-    const uint64_t behind = __builtin_amdgcn_ballot_w64(s < a.b && a.rows[min(s, a.b - 1) + 1] > (int32_t)r);
-    if (behind) return s0 + (uint32_t)__builtin_ctzll(behind);
+  uint32_t s0 = 0;
+  if (a.b > 64) {
+    const uint64_t behind = __builtin_amdgcn_ballot_w64(a.rows[min(64u * (uint32_t)lane_id() + 64u, a.b)] > (int32_t)r);
+    if (!behind) return a.b;
+    s0 = 64 * (uint32_t)__builtin_ctzll(behind);
   }
-  return a.b;
+  const uint32_t s = s0 + lane_id();
+  const uint64_t behind = __builtin_amdgcn_ballot_w64(s < a.b && a.rows[min(s, a.b - 1) + 1] > (int32_t)r);
+  return behind ? s0 + (uint32_t)__builtin_ctzll(behind) : a.b;
 }
 
 // ---- 4 bits -----------------------------------------------------------------
@@ -73,7 +77,8 @@ template <bool V> struct pg_const { static constexpr bool value = V; };
 // A kernel takes the sequences whose columns (rows x the G query heads of a kv
 // head) number more than lo and at most hi, ct columns a tile, and splits each
 // tile's cache rows into chunks of c steps of 64 rows.  Lengths are known on the
-// device only and differ, so c is chosen there, by every wave for itself and from
+// device only and differ, so c is chosen there, by every wave for itself (beyond 64
+// sequences by k_paged_plan, once) and from
 // the same numbers: the smallest of a few tries between all steps / units and all
 // steps / (units - tiles) with which the chunks number at most `units`.  The last
 // try always does (a tile adds one chunk at most to its share); the host launches
@@ -84,7 +89,7 @@ template <bool V> struct pg_const { static constexpr bool value = V; };
 // twice `units` and c at least cbig, it is done again with twice the units: a second
 // round of blocks costs some 7 us and evens out.  `fuse`: the last block of a tile
 // adds its chunks.
-struct PgPlan { uint32_t lo, hi, ct, units, cmin, fuse, slots, cbig; float even; };
+struct PgPlan { uint32_t lo, hi, ct, units, cmin, fuse, slots, cbig; float even; const uint32_t *pre; };
 struct PgUnit { PgSeq q; uint32_t s, tile, chunk, nchunk, c, first, u; };
 
 __device__ __forceinline__ float wave_scan(float v) {           // inclusive, lane order
@@ -97,106 +102,113 @@ __device__ __forceinline__ float wave_scan(float v) {           // inclusive, la
   return v;
 }
 
-// unit u's tile and chunk, or (tiles_only) tile u's first unit; false: none.
-// Counts stay below 2^24 (2^25 heads / ct), exact in f32; the steps' sum need not
-// be.
-__device__ __forceinline__ bool pg_unit(const ThvmPagedArgs &a, const PgPlan &p, uint32_t u, bool tiles_only, PgUnit &o) {
-  const uint32_t lane = lane_id(), G = a.H / a.Hkv;
-  const int32_t cap = (int32_t)(a.maxpages * a.page);
-  // a lane's sequence of each 64: its tiles and steps (the first 64 kept)
-  auto load = [&](uint32_t s0, PgSeq &q, float &tiles, float &steps) {
-    const uint32_t s = s0 + lane;
-    tiles = steps = 0.0f;
-    if (s < a.b) {
-      q = pg_seq(&a, s);
-      const uint32_t rows = (uint32_t)(q.r1 - q.r0), cols = rows * G;
-      if (rows <= a.t && cols > p.lo && cols <= p.hi) tiles = (float)((cols + p.ct - 1) / p.ct);
-      steps = (float)max((min(q.len, cap) + 63) / 64, 1);
-    }
-  };
-  PgSeq q0 = {0, 0, 0}, q;
-  float t0, l0, tl, st;
-  load(0, q0, t0, l0);
-  auto each = [&](auto f) {
-    f(0u, q0, t0, l0);
-    for (uint32_t s0 = 64; s0 < a.b; s0 += 64) {
-      load(s0, q, tl, st);
-      f(s0, q, tl, st);
-    }
-  };
-  float total = 0.0f, tiles = 0.0f;
-  each([&](uint32_t, const PgSeq &, float t, float l) { total += wave_sum(t * l); tiles += wave_sum(t); });
-  if (tiles == 0.0f) return false;
-  // steps in whole chunks of c, and the number with a shorter last one (l < 2^24)
-  auto chunks = [](float l, uint32_t c, float rc, float &full, float &per) {
-    uint32_t q = (uint32_t)(l * rc);
-    int32_t r = (int32_t)((uint32_t)l - q * c);            // q is off by one at most
-    if (r < 0) { q--; r += (int32_t)c; }
-    if (r >= (int32_t)c) { q++; r -= (int32_t)c; }
-    full = (float)q;
-    per = (float)(q + (r != 0));
-  };
+// a sequence's tiles and steps
+__device__ __forceinline__ void pg_count(const ThvmPagedArgs &a, const PgPlan &p, uint32_t s, PgSeq &q, float &tiles, float &steps) {
+  const uint32_t G = a.H / a.Hkv;
+  q = pg_seq(&a, s);
+  const uint32_t rows = (uint32_t)(q.r1 - q.r0), cols = rows * G;
+  tiles = rows <= a.t && cols > p.lo && cols <= p.hi ? (float)((cols + p.ct - 1) / p.ct) : 0.0f;
+  steps = (float)max((min(q.len, (int32_t)(a.maxpages * a.page)) + 63) / 64, 1);
+}
+// steps in whole chunks of c, and the number with a shorter last one (steps < 2^24)
+__device__ __forceinline__ void pg_chunks(float steps, uint32_t c, float &full, float &per) {
+  uint32_t q = (uint32_t)(steps * __builtin_amdgcn_rcpf((float)c));
+  int32_t r = (int32_t)((uint32_t)steps - q * c);          // q is off by one at most
+  if (r < 0) { q--; r += (int32_t)c; }
+  if (r >= (int32_t)c) { q++; r -= (int32_t)c; }
+  full = (float)q;
+  per = (float)(q + (r != 0));
+}
+// c of a plan, and its chunks, all and whole; sum(c, n, whole) adds up both over the
+// sequences.  Counts stay below 2^24 (2^25 heads / ct), exact in f32; the steps' sum
+// need not be.
+template <typename F>
+__device__ __forceinline__ uint32_t pg_choose(const PgPlan &p, float total, float tiles, F sum, float &n, float &whole) {
   uint32_t c;
-  float n, whole;
   for (float units = (float)p.units;; units *= 2.0f) {
     const uint32_t c1 = max(p.cmin, (uint32_t)(total / units)), c2 = max(c1, (uint32_t)(total * 1.0001f / (units - tiles)) + 1);
     c = c1;
     for (int k = 1;; k++) {
-      n = whole = 0.0f;
-      const float rc = __builtin_amdgcn_rcpf((float)c);
-      each([&](uint32_t, const PgSeq &, float t, float l) {
-        float full, per;
-        chunks(l, c, rc, full, per);
-        n += wave_sum(t * per);
-        whole += wave_sum(t * full);
-      });
+      sum(c, n, whole);
       if (n <= units || k > 4) break;
       c = k == 4 ? c2 : c1 + (c2 - c1) * k / 4;
     }
     if (units >= (float)p.slots || c < p.cbig || total >= p.even * units * (float)c) break;
   }
-  if (n > (float)p.slots) return false;                    // row offsets that overlap: nothing is done
-  o.c = c;
+  if (n > (float)p.slots) n = 0.0f;                        // row offsets that overlap: nothing is done
+  return c;
+}
+
+// What k_paged_plan leaves for a batch of more than 64 sequences: c, chunks, whole
+// chunks and tiles in all, then how many tiles, chunks and whole chunks the sequences
+// before each have.
+#define PG_PRE_WORDS(b) (4 + 3 * (((b) + 3) & ~3u))
+
+// unit u's tile and chunk, or (tiles_only) tile u's first unit; false: none
+__device__ __forceinline__ bool pg_unit(const ThvmPagedArgs &a, const PgPlan &p, uint32_t u, bool tiles_only, PgUnit &o) {
+  const uint32_t lane = lane_id(), bb = (a.b + 3) & ~3u;
+  float t = 0.0f, l = 1.0f, n, whole, tiles;
+  PgSeq q = {0, 0, 0};
+  if (p.pre) {
+    const uint4 h = *(const uint4 *)p.pre;
+    o.c = h.x;
+    n = (float)h.y;
+    whole = (float)h.z;
+    tiles = (float)h.w;
+  } else {
+    if (lane < a.b) pg_count(a, p, lane, q, t, l);
+    tiles = wave_sum(t);
+    if (tiles == 0.0f) return false;
+    o.c = pg_choose(p, wave_sum(t * l), tiles, [&](uint32_t c, float &sn, float &sw) {
+      float full, per;
+      pg_chunks(l, c, full, per);
+      sn = wave_sum(t * per);
+      sw = wave_sum(t * full);
+    }, n, whole);
+  }
   // the order of the blocks: whole chunks first, then the tiles' shorter last ones (all
   // of a tile where none is split: backwards, as a prompt's last tiles see most)
-  uint32_t at = u;
-  bool rest = false;
-  if (!tiles_only) {
-    if ((float)u >= n) return false;
-    rest = (float)u >= whole;
-    at = rest ? u - (uint32_t)whole : u;
-    if (whole == 0.0f) at = (uint32_t)n - 1 - u;
+  if (n == 0.0f || (float)u >= (tiles_only ? tiles : n)) return false;
+  const bool rest = !tiles_only && (float)u >= whole;
+  const uint32_t at = tiles_only ? u : whole == 0.0f ? (uint32_t)n - 1 - u : rest ? u - (uint32_t)whole : u;
+  float full, per;
+  uint32_t i, first;                                       // among the sequence's, and its first unit
+  if (p.pre) {
+    const uint32_t *const tb = p.pre + 4, *const nb = tb + bb, *const wb = nb + bb;
+    auto key = [&](uint32_t s) { return tiles_only ? tb[s] : rest ? nb[s] - wb[s] : wb[s]; };
+    // the last sequence with no more before it than at: every 64th, then those between
+    auto last = [&](uint32_t s, uint32_t most) {
+      const uint64_t m = __builtin_amdgcn_ballot_w64(s < most && key(min(s, a.b - 1)) <= at);
+      return 63u - (uint32_t)__builtin_clzll(m | 1);
+    };
+    o.s = 64 * last(64 * lane, a.b);
+    o.s += last(o.s + lane, a.b);
+    pg_count(a, p, o.s, o.q, t, l);
+    pg_chunks(l, o.c, full, per);
+    i = at - key(o.s);
+    first = nb[o.s];
+  } else {
+    pg_chunks(l, o.c, full, per);
+    const float k = tiles_only ? t : t * (rest ? per - full : full), cn = t * per;
+    const float kc = wave_scan(k), nc = wave_scan(cn);
+    const int w = __builtin_ctzll(__builtin_amdgcn_ballot_w64(kc > (float)at) | 1ull << 63);
+    auto get = [&](float v) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), w)); };
+    o.s = w;
+    o.q.r0 = __builtin_amdgcn_readlane(q.r0, w);
+    o.q.r1 = __builtin_amdgcn_readlane(q.r1, w);
+    o.q.len = __builtin_amdgcn_readlane(q.len, w);
+    i = at - (uint32_t)get(kc - k);
+    first = (uint32_t)get(nc - cn);
+    full = get(full);
+    per = get(per);
   }
-  const float rc = __builtin_amdgcn_rcpf((float)c);
-  float before = 0.0f, kbefore = 0.0f;
-  bool found = false;
-  each([&](uint32_t s0, const PgSeq &q, float t, float l) {
-    if (found) return;
-    float full, per;
-    chunks(l, c, rc, full, per);
-    const float n = t * per;
-    const float key = tiles_only ? t : t * (rest ? per - full : full);
-    const float sc = wave_scan(n), kc = wave_scan(key);
-    const uint64_t hit = __builtin_amdgcn_ballot_w64(kbefore + kc > (float)at);
-    if (hit) {
-      const int w = __builtin_ctzll(hit);
-      auto get = [&](float v) { return (uint32_t)__int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), w)); };
-      found = true;
-      o.s = s0 + w;
-      o.q.r0 = __builtin_amdgcn_readlane(q.r0, w);
-      o.q.r1 = __builtin_amdgcn_readlane(q.r1, w);
-      o.q.len = __builtin_amdgcn_readlane(q.len, w);
-      o.nchunk = get(per);
-      const uint32_t i = at - get(kbefore + kc - key), f = get(full);
-      o.tile = tiles_only || rest ? i : i / f;
-      o.chunk = tiles_only ? 0 : rest ? f : i % f;
-      o.first = get(before + sc - n) + o.tile * o.nchunk;
-      o.u = o.first + o.chunk;
-    }
-    before += wave_sum(n);
-    kbefore += wave_sum(key);
-  });
-  return found;
+  const uint32_t f = (uint32_t)full;
+  o.nchunk = (uint32_t)per;
+  o.tile = tiles_only || rest ? i : i / f;
+  o.chunk = tiles_only ? 0 : rest ? f : i % f;
+  o.first = first + o.tile * o.nchunk;
+  o.u = o.first + o.chunk;
+  return true;
 }
 
 typedef void (*paged_fn)(ThvmPagedArgs, PgPlan);
