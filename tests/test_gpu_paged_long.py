@@ -116,6 +116,22 @@ def test_attn_paged_twice_the_chunks(hip, bits, b, ctx):
             assert near(g[row], want, tol, DT_F16), row
 
 
+@pytest.mark.parametrize("dt,bits,hd,page", [(DT_BF16, 16, 128, 32), (DT_F16, 4, 64, 64)])
+@pytest.mark.parametrize("H,Hkv,rows", [(32, 2, 1), (4, 2, 7), (80, 2, 1)])
+def test_attn_paged_merged_columns(hip, dt, bits, hd, page, H, Hkv, rows):
+    """Tiles of 16 columns, many of them, in a few chunks each."""
+    say(f"case: attn_paged merged columns dt={dt} bits={bits} hd={hd} H={H} rows={rows}")
+    P, q, kp, vp, scale = case([(rows, max(rows, 4000 - 97 * i)) for i in range(40)], dt, bits, H, Hkv, hd, page, pages=70)
+    check_attn(P, q, kp, vp, attn(hip, P, q, kp, vp, scale), scale)
+
+
+def test_attn_paged_heads_each_their_own(hip):
+    """Hundreds of kv heads."""
+    say("case: attn_paged of 512 kv heads")
+    P, q, kp, vp, scale = case([(1, 700), (1, 33), (1, 1)], DT_BF16, 16, 512, 512, 64, 64)
+    check_attn(P, q, kp, vp, attn(hip, P, q, kp, vp, scale), scale)
+
+
 PROMPT = {"chunk": [(150, 2500)], "chunks": [(70, 1900), (129, 129), (1, 800), (33, 40)], "even": [(40, 640), (40, 900)]}
 
 

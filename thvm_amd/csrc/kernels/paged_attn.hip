@@ -611,10 +611,11 @@ static paged_fn pa_split(uint32_t cg) {
 }
 struct PaKernels { paged_fn split, merge, tmerge; };
 template <int HD, int XT>
-static PaKernels pa_pick(const ThvmPagedArgs *a, uint32_t cg) {
-  constexpr int NG = 1024 / HD;                            // one column a block
+static PaKernels pa_pick(const ThvmPagedArgs *a, uint32_t cg, uint32_t cb) {
+  constexpr int NG = 1024 / HD;                            // (one column a block: all groups)
   return PaKernels{a->bits == 16 ? pa_split<HD, XT, 16>(cg) : pa_split<HD, XT, 4>(cg),
-                   cg == 4 ? k_paged_merge<HD, XT, 4, NG, 1> : cg == 8 ? k_paged_merge<HD, XT, 8, NG, 1> : k_paged_merge<HD, XT, 16, NG, 1>,
+                   cg == 4 ? k_paged_merge<HD, XT, 4, NG, 1> : cg == 8 ? k_paged_merge<HD, XT, 8, NG, 1>
+                   : cb == 1 ? k_paged_merge<HD, XT, 16, NG, 1> : k_paged_merge<HD, XT, 16, 2, 4>,
                    k_paged_merge<HD, XT, PP_COLS, 1, PA_MERGE>};
 }
 
@@ -623,8 +624,13 @@ extern "C" int thvm_k_attn_paged(const ThvmPagedArgs *call, hipStream_t s, char 
   ThvmPagedArgs args = *call, *const a = &args;
   PaRule r = pa_rule(a);
   const int bf = a->dt == THVM_DT_BF16;
-  const PaKernels k = a->hd == 128 ? (bf ? pa_pick<128, GX_BF16>(a, r.cg) : pa_pick<128, GX_F16>(a, r.cg))
-                                   : (bf ? pa_pick<64, GX_BF16>(a, r.cg) : pa_pick<64, GX_F16>(a, r.cg));
+  // Columns a block of the merge: one, with all its groups on the chunks; of 16 columns
+  // four from 64 tiles on, which have few chunks and would be blocks that plan more than
+  // they add (1 | 4 columns, us: 16 x 8 tiles 27.3 | 25.3, 8 x 8 20.2 | 20.0, one of 4000
+  // rows 14.5 | 16.6)
+  const uint32_t cb = r.cg == 16 && (uint64_t)a->Hkv * r.few_tiles >= 64 ? 4 : 1;
+  const PaKernels k = a->hd == 128 ? (bf ? pa_pick<128, GX_BF16>(a, r.cg, cb) : pa_pick<128, GX_F16>(a, r.cg, cb))
+                                   : (bf ? pa_pick<64, GX_BF16>(a, r.cg, cb) : pa_pick<64, GX_F16>(a, r.cg, cb));
   const bool plan = a->b > 64;
   if (plan) {
     r.fpl.pre = (const uint32_t *)a->ws;
@@ -637,7 +643,7 @@ extern "C" int thvm_k_attn_paged(const ThvmPagedArgs *call, hipStream_t s, char 
     const bool last = !r.many;
     thvm_launch(!plan, last && r.fpl.fuse, k.split, dim3(a->Hkv * r.fpl.slots), dim3(PS_THREADS), 0, s, *a, r.fpl);
     if (!r.fpl.fuse)
-      thvm_launch(false, last, k.merge, dim3(a->Hkv * r.cg * r.few_tiles), dim3(256), 0, s, *a, r.fpl);
+      thvm_launch(false, last, k.merge, dim3(a->Hkv * (r.cg / cb) * r.few_tiles), dim3(256), 0, s, *a, r.fpl);
   }
   if (r.many) {
     thvm_launch(!plan && !r.few, !r.split, pp_tile_pick(a), dim3(a->Hkv * r.mpl.slots), dim3(PP_THREADS), 0, s, *a, r.mpl);
