@@ -112,7 +112,7 @@ static __device__ uint32_t pa_arrived[PA_COUNTERS];
 // the cache's bytes are the bound; its sum, like all else, is f32.
 // Bound by the cache's bytes: over 16 bits 16 requests of 30000 rows (8 kv heads of
 // 128, 4 query heads each) run at 6.4 TB/s, 32 ragged ones of up to 16000 rows at 5.5;
-// over 4 bits 16 of 100000 rows at 5.3 TB/s, where the codec's instructions and the
+// over 4 bits 16 of 100000 rows at 5.5 TB/s, where the codec's instructions and the
 // loads share a SIMD's two waves.  Short contexts: some 7 us of dependent steps (plan,
 // page ids, rows, hand-off), 11 us for one request of 2049 rows.
 #define PS_WAVES 4
@@ -299,6 +299,10 @@ __global__ __launch_bounds__(PS_THREADS, HD == 64 && BITS == 4 ? (CG == 8 ? 3 : 
     place(idn, it + 1);
     idn = ids(it + 2);
     issue_k();
+    // Over 4 bits the SIMD's instructions bound it: the wave at its V goes first, so the
+    // two drift apart and one's scores overlap the other's products (16 requests of
+    // 100000 rows 324 -> 314 us, two 51 -> 49; over 16 bits no change)
+    if constexpr (BITS == 4) __builtin_amdgcn_s_setprio(1);
     // V: 16-bit values of rows 4 lg + j, columns EC lc ..
     uint32_t w[4][4][EC / 2];
     bool odd = false;                                      // a value that is not finite
@@ -415,6 +419,7 @@ __global__ __launch_bounds__(PS_THREADS, HD == 64 && BITS == 4 ? (CG == 8 ? 3 : 
       }
     }
     issue_v();
+    if constexpr (BITS == 4) __builtin_amdgcn_s_setprio(0);
   }
   // the waves (and the column groups) meet in LDS
   l += xor16_f(l);
